@@ -62,6 +62,15 @@ class ExchangeCtx(ctypes.Structure):
                 ("barrier_count", ctypes.c_void_p)]
 
 
+class Kv4Batch(ctypes.Structure):
+    """dq_kv4_batch of the header."""
+    _fields_ = [("pages", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("num_pages", ctypes.c_int64),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("kv_len", ctypes.c_void_p),
+                ("cu_new", ctypes.c_void_p), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32),
+                ("hkv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("pages_per_seq", ctypes.c_int32)]
+
+
 SIGNATURES = {
     "dq_init": (_i, [_i]),
     "dq_last_error_string": (_c.c_char_p, []),
@@ -117,6 +126,11 @@ SIGNATURES = {
     "dq_linear_w4a4_int4_bias": (_i, [_vp, _i64, _vp, _hp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _i, _vp,
                                       _sz, _vp]),
     "dq_rope_kv_append": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "dq_kv4_page_bytes": (_sz, [_i, _i, _i]),
+    "dq_kv4_append": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _vp]),
+    "dq_kv4_read": (_i, [_vp, _vp, _vp, _vp]),
+    "dq_kv4_attention_workspace_bytes": (_sz, [_vp, _i, _i]),
+    "dq_kv4_attention": (_i, [_vp, _vp, _i64, _i64, _i, _i, _i, _i, _c.c_float, _vp, _vp, _sz, _vp]),
     "dq_linear_a16w4_scratch_bytes": (_sz, [_i, _i, _i]),
     "dq_linear_a16w4": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _sz, _vp]),
     "dq_linear_w4a4_int4_static_max_bytes": (_sz, []),

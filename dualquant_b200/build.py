@@ -40,6 +40,8 @@ SOURCES = [
     "gemm_w4a4_int4_f8_out5.cu",
     "gemm_fp4_persist.cu",
     "exchange.cu",
+    "kv4_cache.cu",
+    "kv4_attn_decode.cu",
 ]
 
 NVCC_FLAGS = [

@@ -1,0 +1,287 @@
+// Writing to and reading from the paged 4-bit key/value cache (layout: kv4.cuh).
+//
+// kv4_append_kernel: position rotation of query and key heads, an optional Walsh-Hadamard rotation over the head (the
+// online rotation that keeps outlier channels of keys from setting the grid of a whole head; applied to q and k alike it
+// leaves their products as they are), 4-bit quantisation of keys and values, write into the pages.  All in fp32:
+//   lo = x1 c - x2 s, hi = x2 c + x1 s        x1, x2: the halves of the head; each product and sum rounded on its own
+//   butterflies h = 1, 2, 4 ... d / 2, then times fp32(d^-1/2)
+//   scale = fp16((max - min) * fp32(1 / 15)), zero = fp16(min), code = clamp(rint((x - zero) * (1 / scale)), 0, 15)
+// The two roundings to fp16 are the storage of the grid: codes are taken on the stored grid, and 4 bytes a head against
+// d / 2 of codes are 6 to 12 % of the cache.  NaN is stored as 0 and what fp16 cannot hold as +-65504, so that a page that
+// was written holds finite numbers only.
+#include "kv4.cuh"
+
+namespace dq {
+
+__device__ __forceinline__ void bf16x8_to_float(const uint4& v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[2 * j] = __uint_as_float(w[j] << 16);
+    f[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// d / 16 lanes hold a head: lane l the elements 8l ... 8l + 7 of both halves, so that the rotation of positions, three
+// butterfly stages and the last one stay in registers.  grid: (T, heads / heads per block).
+template <int HD>
+__global__ void __launch_bounds__(128)
+kv4_append_kernel(Kv4Batch c, const unsigned short* qkv, int64_t ld, const float* cos_tab, const float* sin_tab, int tab_rows,
+                  int hq, int rotate, unsigned short* __restrict__ q_out) {
+  grid_dep_launch_dependents();
+  grid_dep_wait();
+  constexpr int LANES = HD / 16, HALF = HD / 2;
+  const int lane = threadIdx.x & 31, l = threadIdx.x % LANES;
+  const int row = blockIdx.x, head = blockIdx.y * (128 / LANES) + threadIdx.x / LANES;
+  const int b = kv4_seq_of_row(c, row, lane);
+  if (b >= c.B) return;
+  const Kv4Seq s = kv4_seq(c, b);
+  if (row < s.row0 || row - s.row0 >= s.n) return;
+  const bool live = head < hq + 2 * c.hkv;  // whole groups of lanes; the shuffles below want every lane
+  const int pos = s.kv - s.n + (row - s.row0);
+  const bool there = pos >= 0 && pos < c.capacity && pos < tab_rows;
+  const bool is_q = head < hq, is_v = head >= hq + c.hkv;
+  float x[16];
+  {
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    if (live) {
+      const unsigned short* src = qkv + row * ld + static_cast<int64_t>(head) * HD + 8 * l;
+      lo = *reinterpret_cast<const uint4*>(src);
+      hi = *reinterpret_cast<const uint4*>(src + HALF);
+    }
+    bf16x8_to_float(lo, x);
+    bf16x8_to_float(hi, x + 8);
+  }
+  if (!is_v && there) {
+    const float4* cp = reinterpret_cast<const float4*>(cos_tab + static_cast<int64_t>(pos) * HALF + 8 * l);
+    const float4* sp = reinterpret_cast<const float4*>(sin_tab + static_cast<int64_t>(pos) * HALF + 8 * l);
+    const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
+    const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = x[j], d = x[j + 8];
+      x[j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(d, sn[j]));
+      x[j + 8] = __fadd_rn(__fmul_rn(d, cs[j]), __fmul_rn(a, sn[j]));
+    }
+  }
+  if (rotate) {
+    // (value heads take part in the shuffles and keep their own numbers)
+    float y[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) y[j] = x[j];
+#pragma unroll
+    for (int h = 1; h < 8; h <<= 1)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if ((j & h) == 0) {
+          const float u = y[j], w = y[j + h];
+          y[j] = __fadd_rn(u, w);
+          y[j + h] = __fsub_rn(u, w);
+        }
+#pragma unroll
+    for (int h = 1; h < LANES; h <<= 1)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float o = __shfl_xor_sync(0xFFFFFFFFu, y[j], h);
+        y[j] = (l & h) ? __fsub_rn(o, y[j]) : __fadd_rn(y[j], o);
+      }
+    const float norm = HD == 128 ? 0.08838834764831845f : 0.125f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float u = y[j], w = y[j + 8];
+      y[j] = __fmul_rn(__fadd_rn(u, w), norm);
+      y[j + 8] = __fmul_rn(__fsub_rn(u, w), norm);
+    }
+    if (!is_v) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = y[j];
+    }
+  }
+  if (is_q) {
+    // a token without a place in the cache has no position: its query row is zero
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = there ? bf16x2_of(x[2 * j], x[2 * j + 1]) : 0u;
+    unsigned short* dst = q_out + (static_cast<int64_t>(row) * hq + head) * HD + 8 * l;
+    if (live) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(dst + HALF) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  float lo = 65504.0f, hi = -65504.0f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    x[j] = isnan(x[j]) ? 0.0f : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+    lo = fminf(lo, x[j]);
+    hi = fmaxf(hi, x[j]);
+  }
+#pragma unroll
+  for (int h = 1; h < LANES; h <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, h));
+    hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, h));
+  }
+  if (is_q || !live || !there) return;
+  const int page = c.table[b * c.table_stride + (pos >> c.page_shift)];
+  if (page < 0 || page >= c.num_pages) return;
+  const __half hs = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), hz = __float2half_rn(lo);
+  const float sf = __half2float(hs), zf = __half2float(hz);
+  const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
+  uint32_t code[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float r = rintf(__fmul_rn(__fsub_rn(x[j], zf), inv));
+    code[j >> 3] |= static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f)) << (4 * (j & 7));
+  }
+  const int P = 1 << c.page_shift, slot = pos & (P - 1), kvh = head - hq - (is_v ? c.hkv : 0);
+  uint8_t* block = c.pages + page * c.page_stride + static_cast<int64_t>(kvh) * P * (HD + 8);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(block + (is_v ? P * HALF : 0) + slot * HALF) + l;
+  dst[0] = code[0];
+  dst[HALF / 8] = code[1];
+  if (l == 0) {
+    __half2* par = reinterpret_cast<__half2*>(block + P * HD + (is_v ? 4 * P : 0)) + slot;
+    *par = __halves2half2(hs, hz);
+  }
+}
+
+// The values of the last n tokens of each sequence as bf16 rows.  A lane makes 16 elements of a key or value head.
+// Rows of tokens that the cache does not hold are zero.  grid: (T, pieces of 128 threads over 2 * hkv * d / 16 lanes).
+template <int HD>
+__global__ void __launch_bounds__(128)
+kv4_read_kernel(Kv4Batch c, unsigned short* __restrict__ k_out, unsigned short* __restrict__ v_out) {
+  grid_dep_launch_dependents();
+  grid_dep_wait();
+  constexpr int LANES = HD / 16;
+  const int lane = threadIdx.x & 31, row = blockIdx.x;
+  const int b = kv4_seq_of_row(c, row, lane);
+  if (b >= c.B) return;
+  const Kv4Seq s = kv4_seq(c, b);
+  if (row < s.row0 || row - s.row0 >= s.n) return;
+  const int unit = blockIdx.y * 128 + threadIdx.x, head = unit / LANES, l = unit % LANES;
+  if (head >= 2 * c.hkv) return;
+  const bool is_v = head >= c.hkv;
+  const int kvh = head - (is_v ? c.hkv : 0);
+  const int pos = s.kv - s.n + (row - s.row0), P = 1 << c.page_shift, slot = pos & (P - 1);
+  uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  int page = -1;
+  if (pos >= 0 && pos < c.capacity) page = c.table[b * c.table_stride + (pos >> c.page_shift)];
+  if (page >= 0 && page < c.num_pages) {
+    const uint8_t* block = c.pages + page * c.page_stride + static_cast<int64_t>(kvh) * P * (HD + 8);
+    const uint2 w = *reinterpret_cast<const uint2*>(block + (is_v ? P * HD / 2 : 0) + slot * (HD / 2) + 8 * l);
+    const float2 sz = __half22float2(*(reinterpret_cast<const __half2*>(block + P * HD + (is_v ? 4 * P : 0)) + slot));
+    const uint32_t word[2] = {w.x, w.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (the product is exact, so contraction into one FMA changes nothing)
+        const float a = static_cast<float>((word[i] >> (8 * j)) & 15u) * sz.x + sz.y;
+        const float d = static_cast<float>((word[i] >> (8 * j + 4)) & 15u) * sz.x + sz.y;
+        r[j] = bf16x2_of(a, d);
+      }
+      o[i] = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+  }
+  unsigned short* dst = (is_v ? v_out : k_out) + (static_cast<int64_t>(row) * c.hkv + kvh) * HD + 16 * l;
+  reinterpret_cast<uint4*>(dst)[0] = o[0];
+  reinterpret_cast<uint4*>(dst)[1] = o[1];
+}
+
+int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out) {
+  DQ_REQUIRE(in != nullptr, DQ_ERR_NULL, "null dq_kv4_batch");
+  DQ_REQUIRE(in->batch >= 0 && in->tokens >= 0, DQ_ERR_SHAPE, "batch=%d tokens=%d", in->batch, in->tokens);
+  DQ_REQUIRE(in->head_dim == 64 || in->head_dim == 128, DQ_ERR_UNSUPPORTED, "head_dim %d: 64 or 128", in->head_dim);
+  DQ_REQUIRE(in->hkv >= 1 && in->hkv <= 1024, DQ_ERR_SHAPE, "hkv=%d", in->hkv);
+  int shift = 4;
+  while (shift < 8 && (1 << shift) != in->page_size) ++shift;
+  DQ_REQUIRE((1 << shift) == in->page_size, DQ_ERR_UNSUPPORTED, "page_size %d: a power of two from 16 to 256", in->page_size);
+  const int64_t block = static_cast<int64_t>(in->page_size) * (in->head_dim + 8);
+  DQ_REQUIRE(in->num_pages >= 0 && in->num_pages < (1ll << 31), DQ_ERR_SHAPE, "num_pages=%lld", (long long)in->num_pages);
+  DQ_REQUIRE(in->page_stride >= block * in->hkv && in->page_stride % 16 == 0, DQ_ERR_ALIGN,
+             "page_stride %lld: a multiple of 16 and at least hkv blocks of %lld", (long long)in->page_stride, (long long)block);
+  DQ_REQUIRE(in->pages_per_seq >= 0 && static_cast<int64_t>(in->pages_per_seq) * in->page_size < (1ll << 30) &&
+                 in->table_stride >= in->pages_per_seq,
+             DQ_ERR_SHAPE, "pages_per_seq=%d table_stride=%lld", in->pages_per_seq, (long long)in->table_stride);
+  if (in->batch > 0 && in->tokens > 0) {
+    DQ_REQUIRE(in->kv_len != nullptr && (in->block_table != nullptr || in->pages_per_seq == 0) &&
+                   (in->pages != nullptr || in->num_pages == 0),
+               DQ_ERR_NULL, "null pointer");
+    DQ_REQUIRE(aligned(in->pages, 16), DQ_ERR_ALIGN, "pages must be 16-byte aligned");
+    DQ_REQUIRE(in->cu_new != nullptr || in->tokens % in->batch == 0, DQ_ERR_SHAPE,
+               "%d rows do not divide by %d sequences", in->tokens, in->batch);
+  }
+  out->pages = static_cast<uint8_t*>(in->pages);
+  out->page_stride = in->page_stride;
+  out->num_pages = in->num_pages;
+  out->table = in->block_table;
+  out->table_stride = in->table_stride;
+  out->kv_len = in->kv_len;
+  out->cu_new = in->cu_new;
+  out->B = in->batch;
+  out->T = in->tokens;
+  out->hkv = in->hkv;
+  out->page_shift = shift;
+  out->capacity = in->pages_per_seq << shift;
+  return DQ_OK;
+}
+
+}  // namespace dq
+
+using namespace dq;
+
+extern "C" size_t dq_kv4_page_bytes(int hkv, int head_dim, int page_size) {
+  if (hkv < 1 || head_dim < 1 || page_size < 1) return 0;
+  return static_cast<size_t>(hkv) * page_size * (head_dim + 8);
+}
+
+extern "C" int dq_kv4_append(const dq_kv4_batch* batch, const void* qkv_bf16, int64_t ld_qkv, const float* cos_tab,
+                             const float* sin_tab, int table_rows, int hq, int rotate, void* q_out_bf16, void* stream) {
+  if (current_state() == nullptr) return DQ_ERR_NOT_INIT;
+  Kv4Batch c;
+  const int rc = kv4_batch_of(batch, &c);
+  if (rc != DQ_OK) return rc;
+  if (c.B == 0 || c.T == 0) return DQ_OK;
+  const int heads = hq + 2 * c.hkv;
+  DQ_REQUIRE(hq >= 1 && hq <= 4096 && table_rows >= 0, DQ_ERR_SHAPE, "hq=%d table_rows=%d", hq, table_rows);
+  DQ_REQUIRE(qkv_bf16 != nullptr && q_out_bf16 != nullptr && (table_rows == 0 || (cos_tab != nullptr && sin_tab != nullptr)),
+             DQ_ERR_NULL, "null pointer");
+  DQ_REQUIRE(ld_qkv >= static_cast<int64_t>(heads) * batch->head_dim, DQ_ERR_SHAPE, "ld_qkv too small");
+  DQ_REQUIRE(ld_qkv % 8 == 0 && aligned(qkv_bf16, 16) && aligned(cos_tab, 16) && aligned(sin_tab, 16) && aligned(q_out_bf16, 16),
+             DQ_ERR_ALIGN, "rows must be 16-byte aligned (ld_qkv a multiple of 8)");
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const auto* x = static_cast<const unsigned short*>(qkv_bf16);
+  auto* q = static_cast<unsigned short*>(q_out_bf16);
+  if (batch->head_dim == 128)
+    DQ_CHECK_CUDA(launch_pdl(kv4_append_kernel<128>, dim3(c.T, (heads + 15) / 16), dim3(128), 0, cs, c, x, ld_qkv, cos_tab,
+                             sin_tab, table_rows, hq, rotate, q));
+  else
+    DQ_CHECK_CUDA(launch_pdl(kv4_append_kernel<64>, dim3(c.T, (heads + 31) / 32), dim3(128), 0, cs, c, x, ld_qkv, cos_tab,
+                             sin_tab, table_rows, hq, rotate, q));
+  return DQ_OK;
+}
+
+extern "C" int dq_kv4_read(const dq_kv4_batch* batch, void* k_out_bf16, void* v_out_bf16, void* stream) {
+  if (current_state() == nullptr) return DQ_ERR_NOT_INIT;
+  Kv4Batch c;
+  const int rc = kv4_batch_of(batch, &c);
+  if (rc != DQ_OK) return rc;
+  if (c.B == 0 || c.T == 0) return DQ_OK;
+  DQ_REQUIRE(k_out_bf16 != nullptr && v_out_bf16 != nullptr, DQ_ERR_NULL, "null pointer");
+  DQ_REQUIRE(aligned(k_out_bf16, 16) && aligned(v_out_bf16, 16), DQ_ERR_ALIGN, "outputs must be 16-byte aligned");
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  auto* k = static_cast<unsigned short*>(k_out_bf16);
+  auto* v = static_cast<unsigned short*>(v_out_bf16);
+  const int lanes = 2 * c.hkv * batch->head_dim / 16;
+  const dim3 grid(c.T, (lanes + 127) / 128);
+  if (batch->head_dim == 128)
+    DQ_CHECK_CUDA(launch_pdl(kv4_read_kernel<128>, grid, dim3(128), 0, cs, c, k, v));
+  else
+    DQ_CHECK_CUDA(launch_pdl(kv4_read_kernel<64>, grid, dim3(128), 0, cs, c, k, v));
+  return DQ_OK;
+}

@@ -27,6 +27,7 @@
 #include <dlfcn.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "../../include/dualquant_b200.h"
@@ -39,7 +40,8 @@ namespace {
   X(dq_gemm_w4a4_int4_ex) X(dq_gemm_w4a4_int4_residual) X(dq_gemm_w4a4_int4_e4m3)                      \
   X(dq_linear_w4a4_int4) X(dq_linear_w4a4_int4_bias) X(dq_linear_w4a4_int4_scratch_bytes)             \
   X(dq_linear_w4a4_int4_prefill_scratch_bytes) X(dq_linear_a16w4) X(dq_linear_a16w4_scratch_bytes)     \
-  X(dq_linear_w4a4_fp4) X(dq_linear_w4a4_fp4_scratch_bytes)
+  X(dq_linear_w4a4_fp4) X(dq_linear_w4a4_fp4_scratch_bytes)                                           \
+  X(dq_kv4_append) X(dq_kv4_read) X(dq_kv4_attention) X(dq_kv4_attention_workspace_bytes)
 #define DQ_DECLARE(name) decltype(&::name) name = nullptr;
 struct Abi {
   DQ_FUNCTIONS(DQ_DECLARE)
@@ -55,7 +57,7 @@ uint64_t g_inited = 0;              // devices ensure_init has been called for
   X(kind) X(had_k) X(had_dim) X(scale) X(had_mat) X(w_packed) X(sw_t) X(N) X(K) X(group) X(codes)       \
   X(sf_atoms) X(tensor_scale) X(fmt) X(_plan) X(act_quant_enabled) X(online_full_had)                  \
   X(online_partial_had) X(had_K) X(act_fmt) X(quantize_bmm_input) X(dtype) X(_buffers) X(act_scale)    \
-  X(_modules) X(layer) X(_parameters) X(bias) X(_packed) X(_packed_fp4) X(name) X(block_size)
+  X(pages) X(head_dim) X(page_size) X(_modules) X(layer) X(_parameters) X(bias) X(_packed) X(_packed_fp4) X(name) X(block_size)
 #define DQ_DECLARE(n) PyObject* n = nullptr;
 struct Names {
   DQ_NAMES(DQ_DECLARE)
@@ -693,6 +695,160 @@ PyObject* perm_forward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------------------------------ paged 4-bit key/value cache
+// (argument meaning: the Python functions of the same names)
+
+const at::Tensor& index_tensor(PyObject* o, const char* what, int dim, int idx) {
+  const at::Tensor& t = tensor(o, what);
+  if (t.scalar_type() != at::kInt || t.dim() != dim || !t.is_cuda() || t.get_device() != idx ||
+      (t.numel() > 0 && t.stride(-1) != 1)) {
+    PyErr_Format(PyExc_ValueError, "%s must be an int32 tensor with %d dimension(s) and unit inner stride on the cache's device",
+                 what, dim);
+    throw PyError();
+  }
+  return t;
+}
+// ops.KV4Cache, block table, lengths and rows -> the ABI's description; makes the cache's device current
+dq_kv4_batch kv4_batch(PyObject* cache, PyObject* table_o, PyObject* len_o, PyObject* cu_o, int64_t tokens, int* device) {
+  Ref pages_o(PyObject_GetAttr(cache, names.pages));
+  const at::Tensor& pages = tensor(pages_o.p, "pages");
+  const int idx = *device = prep(pages);
+  dq_kv4_batch b = {};
+  b.head_dim = static_cast<int32_t>(attr_long(cache, names.head_dim));
+  b.page_size = static_cast<int32_t>(attr_long(cache, names.page_size));
+  if (pages.scalar_type() != at::kByte || pages.dim() != 3 || b.head_dim < 1 || b.page_size < 1 || pages.size(1) < 1 ||
+      pages.size(2) != static_cast<int64_t>(b.page_size) * (b.head_dim + 8) ||
+      (pages.numel() > 0 && (pages.stride(2) != 1 || pages.stride(1) != pages.size(2))))
+    fail(PyExc_ValueError, "pages must be uint8 [num_pages, hkv, page_size * (head_dim + 8)], contiguous within a page");
+  const at::Tensor& table = index_tensor(table_o, "block_table", 2, idx);
+  const at::Tensor& len = index_tensor(len_o, "kv_len", 1, idx);
+  const int64_t B = len.size(0);
+  if (table.size(0) != B) fail(PyExc_ValueError, "block_table and kv_len must have one row per sequence");
+  if (B > INT32_MAX || tokens > INT32_MAX || table.size(1) > INT32_MAX) fail(PyExc_ValueError, "batch or token count too large");
+  if (cu_o != Py_None) {
+    const at::Tensor& cu = index_tensor(cu_o, "cu_new", 1, idx);
+    if (cu.size(0) != B + 1) fail(PyExc_ValueError, "cu_new must have one entry more than there are sequences");
+    b.cu_new = static_cast<const int32_t*>(cu.data_ptr());
+  } else if (B == 0 ? tokens != 0 : tokens % B != 0) {
+    fail(PyExc_ValueError, "without cu_new every sequence has the same number of rows");
+  }
+  b.pages = pages.data_ptr();
+  b.num_pages = pages.size(0);
+  b.page_stride = pages.size(0) > 1 ? pages.stride(0) : pages.size(1) * pages.size(2);
+  b.block_table = static_cast<const int32_t*>(table.data_ptr());
+  b.table_stride = B > 1 ? table.stride(0) : table.size(1);
+  b.kv_len = static_cast<const int32_t*>(len.data_ptr());
+  b.batch = static_cast<int32_t>(B);
+  b.tokens = static_cast<int32_t>(tokens);
+  b.hkv = static_cast<int32_t>(pages.size(1));
+  b.pages_per_seq = static_cast<int32_t>(table.size(1));
+  return b;
+}
+void on_device(const at::Tensor& t, int idx, const char* what) {
+  if (!t.is_cuda() || t.get_device() != idx) {
+    PyErr_Format(PyExc_ValueError, "%s must be on the cache's device", what);
+    throw PyError();
+  }
+}
+
+// kv4_append(qkv, cos_tab, sin_tab, cache, block_table, kv_len, hq, cu_new, rotate) -> q [T, hq, d]
+PyObject* kv4_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  DQ_ARGS(9, "kv4_append");
+  return guarded([&]() {
+    const at::Tensor& xin = tensor(v[0], "qkv");
+    need_2d(xin);
+    int idx;
+    const dq_kv4_batch b = kv4_batch(v[3], v[4], v[5], v[7], xin.size(0), &idx);
+    on_device(xin, idx, "qkv");
+    if (xin.scalar_type() != at::kBFloat16) fail(PyExc_ValueError, "kv4_append expects bf16 rows");
+    const int64_t hq = as_long(v[6]);
+    if (hq < 1 || hq > 4096 || xin.size(1) != (hq + 2 * b.hkv) * b.head_dim)
+      fail(PyExc_ValueError, "qkv must have (hq + 2 hkv) * head_dim columns");
+    const at::Tensor &cos = tensor(v[1], "cos_tab"), &sin = tensor(v[2], "sin_tab");
+    on_device(cos, idx, "cos_tab");
+    on_device(sin, idx, "sin_tab");
+    if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || cos.dim() != 2 || cos.sizes() != sin.sizes() ||
+        cos.size(1) * 2 != b.head_dim || !cos.is_contiguous() || !sin.is_contiguous() || cos.size(0) > INT32_MAX)
+      fail(PyExc_ValueError, "cos_tab and sin_tab must be contiguous fp32 [positions, head_dim / 2]");
+    // the kernel reads rows 16 bytes at a time
+    at::Tensor x = unit_rows(xin);
+    if (row_stride(x) % 8 != 0 || row_stride(x) < x.size(1) || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone(at::MemoryFormat::Contiguous);
+    at::Tensor q = empty({x.size(0), hq, b.head_dim}, at::kBFloat16, idx);
+    check(abi.dq_kv4_append(&b, x.data_ptr(), row_stride(x), static_cast<const float*>(cos.data_ptr()),
+                            static_cast<const float*>(sin.data_ptr()), static_cast<int>(cos.size(0)), static_cast<int>(hq),
+                            v[8] == Py_True, q.data_ptr(), stream_of(idx)),
+          "dq_kv4_append");
+    return wrap(std::move(q));
+  });
+}
+
+// kv4_read(cache, block_table, kv_len, tokens, cu_new) -> (k, v) [T, hkv, d]
+PyObject* kv4_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  DQ_ARGS(5, "kv4_read");
+  return guarded([&]() {
+    const int64_t T = as_long(v[3]);
+    if (T < 0) fail(PyExc_ValueError, "tokens must not be negative");
+    int idx;
+    const dq_kv4_batch b = kv4_batch(v[0], v[1], v[2], v[4], T, &idx);
+    at::Tensor k = empty({T, b.hkv, b.head_dim}, at::kBFloat16, idx), val = empty({T, b.hkv, b.head_dim}, at::kBFloat16, idx);
+    check(abi.dq_kv4_read(&b, k.data_ptr(), val.data_ptr(), stream_of(idx)), "dq_kv4_read");
+    return pair(std::move(k), std::move(val));
+  });
+}
+
+// kv4_attention(q, cache, block_table, kv_len, cu_new, max_new or None, window, sinks, scale or None, out or None) -> [T, hq, d]
+PyObject* kv4_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  DQ_ARGS(10, "kv4_attention");
+  return guarded([&]() {
+    const at::Tensor& qin = tensor(v[0], "q");
+    if (qin.dim() != 3) fail(PyExc_ValueError, "q must be [tokens, query heads, head_dim]");
+    int idx;
+    const int64_t T = qin.size(0), hq = qin.size(1);
+    const dq_kv4_batch b = kv4_batch(v[1], v[2], v[3], v[4], T, &idx);
+    on_device(qin, idx, "q");
+    if (qin.scalar_type() != at::kBFloat16 || qin.size(2) != b.head_dim)
+      fail(PyExc_ValueError, "q must be bf16 [tokens, query heads, head_dim]");
+    if (hq < 1 || hq > 4096 || hq % b.hkv != 0) fail(PyExc_ValueError, "query heads must be a multiple of the key/value heads");
+    long most = b.batch > 0 ? (v[4] == Py_None ? T / b.batch : T) : 0;
+    if (v[5] != Py_None) {
+      most = as_long(v[5]);
+      if (most < 1) fail(PyExc_ValueError, "max_new must be positive");
+    }
+    const long window = as_long(v[6]), sinks = as_long(v[7]);
+    if (window < 0 || sinks < 0 || window > INT32_MAX || sinks > INT32_MAX)
+      fail(PyExc_ValueError, "window and sinks must be 32-bit and not negative");
+    double scale = 1.0 / std::sqrt(static_cast<double>(b.head_dim));
+    if (v[8] != Py_None) {
+      scale = PyFloat_AsDouble(v[8]);
+      if (PyErr_Occurred()) throw PyError();
+      if (!std::isfinite(static_cast<float>(scale))) fail(PyExc_ValueError, "scale must be finite");
+    }
+    // the kernel reads heads 16 bytes at a time
+    at::Tensor q = unit_rows(qin);
+    if (q.stride(0) % 8 != 0 || q.stride(1) % 8 != 0 || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
+      q = q.clone(at::MemoryFormat::Contiguous);
+    at::Tensor out;
+    if (v[9] != Py_None) {
+      out = tensor(v[9], "out");
+      on_device(out, idx, "out");
+      if (out.scalar_type() != at::kBFloat16 || out.sizes() != qin.sizes() || !out.is_contiguous())
+        fail(PyExc_ValueError, "out must be a contiguous bf16 tensor of q's shape");
+      if (out.numel() > 0 && out.storage().data_ptr().get() == q.storage().data_ptr().get())
+        fail(PyExc_ValueError, "out must not share memory with q");
+    } else {
+      out = empty({T, hq, b.head_dim}, at::kBFloat16, idx);
+    }
+    if (T == 0 || b.batch == 0) return wrap(std::move(out));
+    const int rows = static_cast<int>(std::min<long>(std::max<long>(most, 1), T));
+    const Scratch ws(std::max<int64_t>(static_cast<int64_t>(abi.dq_kv4_attention_workspace_bytes(&b, static_cast<int>(hq), rows)), 256));
+    check(abi.dq_kv4_attention(&b, q.data_ptr(), q.stride(0), q.stride(1), static_cast<int>(hq), rows, static_cast<int>(window),
+                               static_cast<int>(sinks), static_cast<float>(scale), out.data_ptr(), ws.mem.get(), ws.bytes,
+                               stream_of(idx)),
+          "dq_kv4_attention");
+    return wrap(std::move(out));
+  });
+}
+
 // ------------------------------------------------------------------------------------ module
 // setup(library path, check, ensure_init)
 PyObject* setup(PyObject*, PyObject* const* v, Py_ssize_t n) {
@@ -725,6 +881,9 @@ PyMethodDef methods[] = {DQ_METHOD(setup),
                          DQ_METHOD(linear_w4a4_int4),
                          DQ_METHOD(linear_a16w4),
                          DQ_METHOD(linear_w4a4_fp4),
+                         DQ_METHOD(kv4_append),
+                         DQ_METHOD(kv4_read),
+                         DQ_METHOD(kv4_attention),
                          DQ_METHOD(make_plan),
                          DQ_METHOD(perm_forward),
                          {nullptr, nullptr, 0, nullptr}};

@@ -639,3 +639,62 @@ def rope_kv_append(qkv: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tens
                                      _stream(qkv.device)),
                "dq_rope_kv_append")
     return q.transpose(1, 2)
+
+
+# ---------------------------------------------------------------------------------------------
+# paged key/value cache in 4 bits
+# ---------------------------------------------------------------------------------------------
+@dataclass
+class KV4Cache:
+    """Pages of one layer's key/value cache, 4 bits per element: uint8 [num_pages, hkv, page_size * (head_dim + 8)].
+    The block of a head holds key codes [page_size, head_dim / 2] (element 2i in the low half of byte i), value codes, and
+    fp16 (scale, zero) pairs of keys and of values [page_size, 2]; a code c stands for scale * c + zero.  head_dim 64 or 128,
+    page_size a power of two from 16 to 256.  `pages` may be a slice of a larger tensor (one layer of [pages, layers, ...])."""
+
+    pages: torch.Tensor
+    head_dim: int
+    page_size: int
+
+    @property
+    def hkv(self) -> int:
+        return self.pages.shape[1]
+
+
+def kv4_cache(num_pages: int, hkv: int, head_dim: int, page_size: int = 64, device="cuda") -> KV4Cache:
+    """An empty cache of num_pages pages."""
+    if head_dim not in (64, 128) or page_size not in (16, 32, 64, 128, 256) or num_pages < 0 or hkv < 1:
+        raise ValueError("head_dim must be 64 or 128, page_size a power of two from 16 to 256")
+    return KV4Cache(torch.zeros(num_pages, hkv, page_size * (head_dim + 8), dtype=torch.uint8, device=device), head_dim,
+                    page_size)
+
+
+def kv4_append(qkv: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tensor, cache: KV4Cache,
+               block_table: torch.Tensor, kv_len: torch.Tensor, hq: int, cu_new: Optional[torch.Tensor] = None,
+               rotate: bool = True) -> torch.Tensor:
+    """New tokens of a ragged batch into the paged 4-bit cache: qkv [T, (hq + 2 hkv) * d] bf16 -> rotated queries [T, hq, d].
+
+    block_table int32 [B, pages per sequence]; kv_len int32 [B]: tokens of each sequence with the new ones; cu_new int32 [B + 1]:
+    first row of each sequence's new tokens (None: T / B rows each).  Row i of a sequence with n new tokens goes to position
+    kv_len - n + i.  cos_tab / sin_tab fp32 [positions, d / 2].  rotate: a normalised Walsh-Hadamard rotation over the head of
+    queries and keys behind the position rotation, which spreads outlier channels of keys over the 4-bit grid and leaves
+    q . k as it is.  All index tensors are read on the device; rows from cu_new[B] on are left as they were.  A token without
+    a place (negative position, behind the table row or the rotation tables) gets a zero query row and is not written, nor is
+    one whose page number lies outside of the cache."""
+    return _lib.host().kv4_append(qkv, cos_tab, sin_tab, cache, block_table, kv_len, hq, cu_new, bool(rotate))
+
+
+def kv4_read(cache: KV4Cache, block_table: torch.Tensor, kv_len: torch.Tensor, tokens: int,
+             cu_new: Optional[torch.Tensor] = None):
+    """What the cache holds for the last tokens of each sequence (rows as in kv4_append, `tokens` of them in all):
+    (keys, values) bf16 [tokens, hkv, d], keys as they were stored (rotated).  Tokens that are not there are zero."""
+    return _lib.host().kv4_read(cache, block_table, kv_len, tokens, cu_new)
+
+
+def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, kv_len: torch.Tensor,
+                  cu_new: Optional[torch.Tensor] = None, max_new: Optional[int] = None, window: int = 0, sinks: int = 0,
+                  scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal grouped-query attention of the new tokens (q [T, hq, d] bf16, rows as in kv4_append) over the paged 4-bit cache:
+    bf16 [T, hq, d].  window > 0: a token sees itself, the window - 1 tokens before it and the first `sinks` tokens of its
+    sequence.  scale: default d ** -0.5.  max_new: the most rows that a sequence brings, which chooses the kernel; T (or T / B
+    without cu_new) if not given.  A row that sees no token is zero; rows from cu_new[B] on are not written."""
+    return _lib.host().kv4_attention(q, cache, block_table, kv_len, cu_new, max_new, window, sinks, scale, out)

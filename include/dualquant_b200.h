@@ -582,6 +582,52 @@ DQ_API int dq_linear_w4a4_int4_static(const void* x_bf16, int64_t ldx, const flo
                                       const void* sw_t, const float* r, int M, int N, int K,
                                       int G, void* y, int y_dtype, int scale_fp16, void* stream);
 
+/* ---- paged key/value cache in 4 bits ------------------------------------------------------
+ * No counterpart in the reference, which leaves attention and its cache to the HF decoder layer that it wraps.
+ *
+ * A page holds page_size tokens (16, 32, 64, 128 or 256) of every key/value head; the block of one head is
+ * page_size * (head_dim + 8) bytes (head_dim 64 or 128):
+ *   key codes [page_size][head_dim / 2]   element 2i of the head in the low half of byte i, 2i + 1 in the high half
+ *   value codes [page_size][head_dim / 2]
+ *   key (scale, zero) [page_size][2] fp16, value (scale, zero) [page_size][2] fp16
+ * A code c stands for scale * c + zero.  Pages of one layer: [num_pages][hkv blocks], page_stride bytes apart.
+ */
+typedef struct dq_kv4_batch {
+  void* pages;                 /* 16-byte aligned                                                       */
+  int64_t page_stride;         /* bytes from page to page, a multiple of 16                             */
+  int64_t num_pages;
+  const int32_t* block_table;  /* [batch][table_stride]: page of a sequence's tokens i * page_size ...; an entry
+                                  outside [0, num_pages) is a page that is not there                    */
+  int64_t table_stride;
+  const int32_t* kv_len;       /* [batch] tokens of a sequence, the new ones included                   */
+  const int32_t* cu_new;       /* [batch + 1] first row of a sequence's new tokens; NULL: tokens / batch each */
+  int32_t batch;
+  int32_t tokens;              /* rows of the call's tensors; rows from cu_new[batch] on are left alone */
+  int32_t hkv, head_dim, page_size;
+  int32_t pages_per_seq;       /* entries of a table row                                                */
+} dq_kv4_batch;
+/* Row i of a sequence with n new tokens is the token at position kv_len - n + i.  Lengths and tables are read on the
+ * device, so that the calls can be captured and replayed with others. */
+
+DQ_API size_t dq_kv4_page_bytes(int hkv, int head_dim, int page_size);
+/* New tokens into the cache: qkv [tokens][(hq + 2 hkv) * head_dim] bf16; position rotation of query and key heads from fp32
+ * tables [table_rows][head_dim / 2], with rotate != 0 a normalised Walsh-Hadamard rotation of both over the head, 4-bit
+ * quantisation of keys and values (scale fp16((max - min) / 15), zero fp16(min); NaN as 0, +-65504 at most).  q_out
+ * [tokens][hq][head_dim] bf16 gets the rotated queries.  A token whose position is negative, behind the table row or behind
+ * the rotation tables is not written and has a zero query row; one whose page is not there is not written. */
+DQ_API int dq_kv4_append(const dq_kv4_batch* batch, const void* qkv_bf16, int64_t ld_qkv, const float* cos_tab,
+                         const float* sin_tab, int table_rows, int hq, int rotate, void* q_out_bf16, void* stream);
+/* The values of the last n tokens of every sequence, as bf16 rows [tokens][hkv][head_dim]; tokens that are not there: 0. */
+DQ_API int dq_kv4_read(const dq_kv4_batch* batch, void* k_out_bf16, void* v_out_bf16, void* stream);
+/* Causal attention of the new tokens over the cache: hq query heads in groups of hq / hkv, q [tokens][hq][head_dim] bf16 with
+ * the given strides (elements).  window > 0: a token sees itself, the window - 1 tokens before it and the first `sinks`
+ * tokens of its sequence.  max_new: no sequence brings more rows (a hint; more are computed all the same).  A row that sees
+ * nothing is zero.  out [tokens][hq][head_dim] bf16. */
+DQ_API size_t dq_kv4_attention_workspace_bytes(const dq_kv4_batch* batch, int hq, int max_new);
+DQ_API int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, int64_t q_row_stride, int64_t q_head_stride,
+                            int hq, int max_new, int window, int sinks, float scale, void* out_bf16, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
