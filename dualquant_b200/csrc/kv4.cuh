@@ -16,6 +16,22 @@ namespace dq {
 
 constexpr int kKv4Far = 1 << 30;  // positions, windows and sinks are cut here: sums of two of them stay in 32 bits
 
+// Division by a number that the host knows: a product and a shift instead of the 150 cycles of an integer division, of which
+// looking up a CTA's share alone took nine in a row.  n in [0, 2^31).
+struct Kv4Div {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+};
+inline Kv4Div kv4_div(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  // 2^31 <= mul < 2^32 for every d, and n * (mul * d - 2^(31 + s)) < 2^(31 + s): exact
+  return {static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint32_t>(d) + 1), 31 + s};
+}
+
 struct Kv4Batch {
   uint8_t* pages;
   int64_t page_stride;      // bytes from page to page
@@ -68,6 +84,11 @@ struct Kv4Mask {
   int window, sinks;  // window 0: no window
 };
 
+struct Kv4Group {  // query heads of a key/value head
+  int G;
+  Kv4Div by;
+};
+
 struct Kv4Span {      // token tiles of a segment
   int count;          // at least one: a segment whose rows see nothing still has its rows written
   int sink_tiles, first;
@@ -76,10 +97,10 @@ struct Kv4Span {      // token tiles of a segment
 };
 
 template <int TK>
-__device__ __forceinline__ Kv4Span kv4_span(const Kv4Batch& c, const Kv4Seq& s, const Kv4Mask& m, int G, int row_tile, int R) {
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Batch& c, const Kv4Seq& s, const Kv4Mask& m, const Kv4Group& g, int row_tile, int R) {
   Kv4Span r;
-  const int rows = s.n * G;
-  const int i0 = row_tile * R / G, i1 = (min((row_tile + 1) * R, rows) - 1) / G;
+  const int rows = s.n * g.G;
+  const int i0 = g.by(row_tile * R), i1 = g.by(min((row_tile + 1) * R, rows) - 1);
   r.p_lo = s.kv - s.n + i0;
   r.p_hi = s.kv - s.n + i1;
   const int hi = min(min(r.p_hi + 1, s.kv), c.capacity);
@@ -98,13 +119,14 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Batch& c, const Kv4Seq& s, 
   return r;
 }
 
-__device__ __forceinline__ int kv4_row_tiles(const Kv4Seq& s, int G, int R) { return (s.n * G + R - 1) / R; }
+__device__ __forceinline__ int kv4_row_tiles(const Kv4Seq& s, const Kv4Group& g, int R) { return (s.n * g.G + R - 1) / R; }
 
 template <int TK>
-__device__ __forceinline__ long long kv4_units_per_head(const Kv4Batch& c, const Kv4Seq& s, const Kv4Mask& m, int G, int R) {
-  long long n = 0;
-  const int tiles = kv4_row_tiles(s, G, R);
-  for (int rt = 0; rt < tiles; ++rt) n += kv4_span<TK>(c, s, m, G, rt, R).count;
+__device__ __forceinline__ int kv4_units_per_head(const Kv4Batch& c, const Kv4Seq& s, const Kv4Mask& m, const Kv4Group& g, int R) {
+  int n = 0;
+  const int tiles = kv4_row_tiles(s, g, R);
+#pragma unroll 1
+  for (int rt = 0; rt < tiles; ++rt) n += kv4_span<TK>(c, s, m, g, rt, R).count;
   return n;
 }
 
@@ -113,15 +135,15 @@ struct Kv4Cursor {
   int b, h, rt;
   Kv4Seq seq;
   Kv4Span span;
-  int u0, u1;      // this CTA's tiles of the segment
-  long long left;  // tiles of the CTA behind this segment
+  int u0, u1;  // this CTA's tiles of the segment
+  int left;    // tiles of the CTA behind this segment
 };
 
 // Steps over to the next segment that has tiles; false: none of the CTA's tiles are left.
 template <int TK>
-__device__ __forceinline__ bool kv4_next_segment(const Kv4Batch& c, const Kv4Mask& m, int G, int R, Kv4Cursor& k) {
+__device__ __forceinline__ bool kv4_next_segment(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, Kv4Cursor& k) {
   if (k.left <= 0) return false;
-  if (++k.rt >= kv4_row_tiles(k.seq, G, R)) {
+  if (++k.rt >= kv4_row_tiles(k.seq, g, R)) {
     k.rt = 0;
     if (++k.h >= c.hkv) {
       k.h = 0;
@@ -131,95 +153,168 @@ __device__ __forceinline__ bool kv4_next_segment(const Kv4Batch& c, const Kv4Mas
       } while (k.seq.n == 0);
     }
   }
-  k.span = kv4_span<TK>(c, k.seq, m, G, k.rt, R);
+  k.span = kv4_span<TK>(c, k.seq, m, g, k.rt, R);
   k.u0 = 0;
-  k.u1 = static_cast<int>(min(static_cast<long long>(k.span.count), k.left));
+  k.u1 = min(k.span.count, k.left);
   k.left -= k.u1;
   return true;
 }
 
-struct Kv4Share {
-  long long total, share;  // tiles of the call, tiles of a CTA
+struct Kv4Start {
+  Kv4Cursor k;  // the CTA's first segment
+  int share;    // tiles of every CTA
+  bool any;     // false: the CTA has no tile
 };
-
-// Whole block of THREADS threads.  s_scan: THREADS + 1 long longs.  least: tiles that a CTA takes at least.
-template <int TK, int THREADS>
-__device__ __forceinline__ long long kv4_scan_units(const Kv4Batch& c, const Kv4Mask& m, int G, int R, int base,
-                                                    long long* s_scan) {
-  const int b = base + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long n = 0;
-  if (b < c.B) {
-    const Kv4Seq s = kv4_seq(c, b);
-    n = c.hkv * kv4_units_per_head<TK>(c, s, m, G, R);
-  }
+// Finds a CTA's share of the line and its first segment.  One warp.  grid: divides by gridDim.x; least: tiles a CTA takes at
+// least.  Tile numbers are 32-bit; the host refuses batches that could pass that.
+//
+// The instructions of a kernel are cold when it starts (a pass through kv4_begin_any took 5000 cycles, a second one 1400), and
+// what is read ahead ends at the next jump: batches of up to 128 sequences with one row tile each, the decode step, have a path
+// without a loop, all others a function of their own.
+__device__ __forceinline__ int kv4_warp_scan(int v, int lane) {
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long v = __shfl_up_sync(0xFFFFFFFFu, n, d);
-    if (lane >= d) n += v;
+    const int o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+    if (lane >= d) v += o;
   }
-  __shared__ long long s_warp[THREADS / 32];
-  __syncthreads();
-  if (lane == 31) s_warp[warp] = n;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) n += s_warp[w];
-  s_scan[threadIdx.x + 1] = n;
-  if (threadIdx.x == 0) s_scan[0] = 0;
-  __syncthreads();
-  return s_scan[THREADS];
+  return v;
+}
+__device__ __forceinline__ int kv4_share_of(int total, int least, Kv4Div grid) {
+  // (the sum passes 31 bits for a total within gridDim.x of 2^31)
+  const int g = static_cast<int>(gridDim.x);
+  return max(total < 0x7FFF0000 ? grid(total + g - 1) : total / g + 1, least);
+}
+// in / per_head, below 1024: the quotient of floats is off by less than one
+__device__ __forceinline__ int kv4_head_of(int in, int per_head) {
+  int h = static_cast<int>(__fdividef(static_cast<float>(in), static_cast<float>(per_head)));
+  if (h * per_head > in) --h;
+  if ((h + 1) * per_head <= in) ++h;
+  return h;
 }
 
-template <int TK, int THREADS>
-__device__ __forceinline__ Kv4Share kv4_share(const Kv4Batch& c, const Kv4Mask& m, int G, int R, int least, long long* s_scan) {
-  Kv4Share r;
-  r.total = 0;
-  for (int base = 0; base < c.B; base += THREADS) r.total += kv4_scan_units<TK, THREADS>(c, m, G, R, base, s_scan);
-  r.share = (r.total + gridDim.x - 1) / gridDim.x;
-  if (r.share < least) r.share = least;
-  return r;
-}
-
-// The segment that holds tile `at` (< total), with the tiles [at, at + want) of it and behind it.  Returns the number of the
-// segment's first tile on the line.  Whole block; s_scan as kv4_share left it (its last round of sequences).
-template <int TK, int THREADS>
-__device__ __forceinline__ long long kv4_locate(const Kv4Batch& c, const Kv4Mask& m, int G, int R, long long at, long long want,
-                                                long long* s_scan, Kv4Cursor& k) {
-  long long before = 0;
-  int base = 0;
-  if (c.B > THREADS) {
-    for (;; base += THREADS) {
-      const long long n = kv4_scan_units<TK, THREADS>(c, m, G, R, base, s_scan);
-      if (before + n > at || base + THREADS >= c.B) break;
-      before += n;
-    }
+// Any batch: a lane adds up B / 32 neighbouring sequences, and the sequences of the lane that holds the first tile are added up
+// once more, one a lane (two rounds of loads for up to 1024).
+template <int TK>
+__device__ __noinline__ Kv4Start kv4_begin_any(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, int least,
+                                               Kv4Div grid, int lane) {
+  Kv4Start r;
+  Kv4Cursor& k = r.k;
+  const int each = (c.B + 31) / 32;
+  int n = 0;
+#pragma unroll 1
+  for (int i = 0; i < each; ++i) {
+    const int b = lane * each + i;
+    if (b < c.B) n += kv4_units_per_head<TK>(c, kv4_seq(c, b), m, g, R) * c.hkv;
   }
-  const long long rest = at - before;
-  int lo = 0, hi = THREADS - 1;  // the last sequence whose tiles begin at or before `rest`: empty ones share a beginning
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s_scan[mid] <= rest) lo = mid;
-    else hi = mid - 1;
+  const int upto = kv4_warp_scan(n, lane), total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+  r.share = kv4_share_of(total, least, grid);
+  const long long at = static_cast<long long>(blockIdx.x) * r.share;
+  r.any = at < total;
+  if (!r.any) return r;
+  const int begin = static_cast<int>(at);
+  int owner = __ffs(__ballot_sync(0xFFFFFFFFu, upto > begin)) - 1;
+  int in = begin - __shfl_sync(0xFFFFFFFFu, upto - n, owner);
+  k.b = owner * each;
+  int per_head = 0, u = 0, v = 0;
+  uint32_t past = 0;
+#pragma unroll 1
+  for (int base = 0; base < each; base += 32) {
+    const int b = owner * each + base + lane;
+    per_head = 0;
+    if (base + lane < each && b < c.B) per_head = kv4_units_per_head<TK>(c, kv4_seq(c, b), m, g, R);
+    v = per_head * c.hkv;
+    u = kv4_warp_scan(v, lane);
+    past = __ballot_sync(0xFFFFFFFFu, u > in);
+    if (past != 0) break;  // (one of them holds the tile)
+    k.b += 32;
+    in -= __shfl_sync(0xFFFFFFFFu, u, 31);
   }
-  k.b = base + lo;
+  owner = (__ffs(past) - 1) & 31;
+  k.b += owner;
+  in -= __shfl_sync(0xFFFFFFFFu, u - v, owner);
+  per_head = __shfl_sync(0xFFFFFFFFu, per_head, owner);
   k.seq = kv4_seq(c, k.b);
-  long long in = rest - s_scan[lo];
-  const long long per_head = (s_scan[lo + 1] - s_scan[lo]) / c.hkv;
-  k.h = static_cast<int>(in / per_head);
+  k.h = kv4_head_of(in, per_head);
   in -= k.h * per_head;
   k.rt = 0;
-  k.span = kv4_span<TK>(c, k.seq, m, G, 0, R);
+  k.span = kv4_span<TK>(c, k.seq, m, g, 0, R);
+#pragma unroll 1
   while (in >= k.span.count) {
     in -= k.span.count;
     ++k.rt;
-    k.span = kv4_span<TK>(c, k.seq, m, G, k.rt, R);
+    k.span = kv4_span<TK>(c, k.seq, m, g, k.rt, R);
   }
-  k.u0 = static_cast<int>(in);
-  k.u1 = static_cast<int>(min(static_cast<long long>(k.span.count), in + want));
+  const int want = min(r.share, total - begin);
+  k.u0 = in;
+  k.u1 = min(k.span.count, in + want);
   k.left = want - (k.u1 - k.u0);
-  return at - in;
+  return r;
 }
 
-// Sums of a segment that a CTA shares with others: [cta][0: its first segment, 1: its last][R rows: m, l, then O[d]]
+template <int TK>
+__device__ __forceinline__ Kv4Start kv4_begin(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, int least, Kv4Div grid,
+                                              int lane) {
+  constexpr int N = 4;  // sequences of a lane
+  const int each = c.B <= 32 ? 1 : N;
+  Kv4Seq seq[N];
+  bool one = c.B <= 32 * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    seq[i] = {0, 0, 0};
+    const int b = lane * each + i;
+    if (i < each && b < c.B) seq[i] = kv4_seq(c, b);
+    one &= seq[i].n * g.G <= R;
+  }
+  if (!__all_sync(0xFFFFFFFFu, one)) return kv4_begin_any<TK>(c, m, g, R, least, grid, lane);
+  Kv4Start r;
+  int upto[N], n = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (seq[i].n > 0) n += kv4_span<TK>(c, seq[i], m, g, 0, R).count * c.hkv;
+    upto[i] = n;
+  }
+  const int all = kv4_warp_scan(n, lane), total = __shfl_sync(0xFFFFFFFFu, all, 31);
+  r.share = kv4_share_of(total, least, grid);
+  const long long at = static_cast<long long>(blockIdx.x) * r.share;
+  r.any = at < total;
+  const int begin = static_cast<int>(at);
+  const int owner = (__ffs(__ballot_sync(0xFFFFFFFFu, all > begin)) - 1) & 31;
+  int in = begin - (all - n), which = 0;  // of use in the owner
+  Kv4Seq s = seq[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i)
+    if (in >= upto[i - 1]) {
+      s = seq[i];
+      which = i;
+    }
+#pragma unroll
+  for (int i = N - 1; i > 0; --i)
+    if (which == i) in -= upto[i - 1];
+  Kv4Cursor& k = r.k;
+  in = __shfl_sync(0xFFFFFFFFu, in, owner);
+  k.b = owner * each + __shfl_sync(0xFFFFFFFFu, which, owner);
+  k.rt = 0;
+  k.seq.row0 = __shfl_sync(0xFFFFFFFFu, s.row0, owner);
+  k.seq.n = __shfl_sync(0xFFFFFFFFu, s.n, owner);
+  k.seq.kv = __shfl_sync(0xFFFFFFFFu, s.kv, owner);
+  k.span = kv4_span<TK>(c, k.seq, m, g, 0, R);
+  k.h = kv4_head_of(in, k.span.count);
+  const int want = min(r.share, total - begin);
+  k.u0 = in - k.h * k.span.count;
+  k.u1 = min(k.span.count, k.u0 + want);
+  k.left = want - (k.u1 - k.u0);
+  return r;
+}
+
+// Workspace: a Kv4Join for every CTA, then the sums of segments that it shares with others, [cta][0: its first segment, 1: its
+// last][m, l of R rows, then O of R rows].
+struct Kv4Join {
+  int parts;     // CTAs from this one on that hold a part of the segment which begins in this one; 0: none goes on
+  int slot;      // where this CTA's part is
+  int rows, first_row, row0, h;
+};
 __host__ __device__ constexpr size_t kv4_partial_floats(int R, int hd) { return static_cast<size_t>(R) * (hd + 2); }
+__host__ __device__ constexpr size_t kv4_join_bytes(int grid) { return (static_cast<size_t>(grid) * sizeof(Kv4Join) + 255) / 256 * 256; }
 
 int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out);
 
@@ -229,8 +324,10 @@ struct Kv4AttnArgs {
   const unsigned short* q;  // bf16
   int64_t q_row, q_head;    // strides in elements
   unsigned short* out;      // bf16 [T][hq][d]
+  Kv4Join* join;
   float* partial;
-  int G;
+  Kv4Group g;
+  Kv4Div grid;              // by the number of CTAs
   float scale2;             // softmax scale * log2(e)
 };
 

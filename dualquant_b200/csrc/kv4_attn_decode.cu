@@ -26,9 +26,14 @@ namespace dq {
 constexpr int kDecTile = 32;     // tokens per tile
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
-constexpr int kDecStages = 3;    // tiles in flight per warp
+constexpr int kDecStages = 2;    // tiles of a warp's ring
+constexpr int kPieces = kDecTile / 16;
+constexpr int kDecQueries = kDecStages + 1;  // query rows of a segment are copied when its predecessor's last tile is
 constexpr int kDecLeast = 4;     // tiles that a CTA takes at least
 constexpr float kNoMax = -1e30f;
+
+template <int HD>
+constexpr int kQPitch = 2 * HD + 16;  // bytes
 
 template <int HD, int NT>
 struct DecSmem {
@@ -37,10 +42,12 @@ struct DecSmem {
   static constexpr int kPitch = HD + 8;  // floats per row of a warp's output in the meeting place
   static constexpr int kOffMeet = kDecWarps * kDecStages * kStage;
   static constexpr int kOffMl = kOffMeet + kDecWarps * R * kPitch * 4;
-  static constexpr int kOffScan = kOffMl + kDecWarps * R * 2 * 4;
-  static constexpr int kOffBar = kOffScan + (kDecThreads + 1) * 8;
-  static constexpr int kOffValid = kOffBar + kDecWarps * kDecStages * 8;
-  static constexpr int kBytes = kOffValid + kDecWarps * kDecStages * 4;
+  static constexpr int kQBytes = R * kQPitch<HD>;
+  static constexpr int kOffQ = kOffMl + kDecWarps * R * 2 * 4;
+  static constexpr int kOffValid = kOffQ + kDecQueries * kQBytes;
+  static constexpr int kOffCursor = kOffValid + kDecWarps * kDecStages * 4;
+  static constexpr int kBytes = kOffCursor + static_cast<int>(sizeof(Kv4Cursor)) + 8;
+  static_assert(kOffQ % 16 == 0 && kOffCursor % 4 == 0, "alignment");
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -63,62 +70,66 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float bf16_float(uint32_t bits) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool is) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The query rows of a segment as the second operand of S' = K Q'.
 template <int HD, int NT>
 struct DecQuery {
   static constexpr int KS = HD / 16;  // steps of 16 head elements
   uint32_t f[NT][KS][2];
-  float zq[NT][2];   // sum of the row's elements, times scale log2(e); NaN for a row that is not finite
+  float2 zq[NT];     // sum of a row's elements, times scale log2(e); NaN for a row that is not finite
   int pos[NT][2];    // the row's position; -1: no such row
   float mul;         // what S' has to be multiplied with to be scores in base 2
 
-  __device__ __forceinline__ void load(const Kv4AttnArgs& a, const Kv4Cursor& k, int lane) {
+  // rows: the segment's query rows in shared memory, bf16, kQPitch bytes apart; rows that do not exist are zero
+  __device__ __forceinline__ void load(const Kv4AttnArgs& a, const Kv4Cursor& k, const uint8_t* q_rows, int lane) {
     constexpr int R = 8 * NT, W = HD / 32;  // W: 32-bit words of codes per lane
-    const int g = lane >> 2, t = lane & 3, rows = k.seq.n * a.G;
-    float q[NT][W * 8];
-    float top = 0.0f, sum[NT];
+    const int g = lane >> 2, t = lane & 3, rows = k.seq.n * a.g.G;
+    uint32_t raw[NT][W * 4];  // pairs of bf16
+    uint32_t top = 0;         // largest size of an element, as bf16 bits
+    float sum[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = k.rt * R + nt * 8 + g;
-      const bool there = r < rows;
-      const int i = there ? r / a.G : 0, head = k.h * a.G + (there ? r - i * a.G : 0);
-      const unsigned short* src =
-          a.q + static_cast<int64_t>(k.seq.row0 + i) * a.q_row + static_cast<int64_t>(head) * a.q_head + t * (W * 8);
+      const uint8_t* src = q_rows + (nt * 8 + g) * kQPitch<HD> + t * (W * 16);
+      uint32_t big = 0;
+      float2 s[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (there) v = *reinterpret_cast<const uint4*>(src + 8 * w);
+        const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * w);
         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          q[nt][8 * w + 2 * j] = __uint_as_float(u[j] << 16);
-          q[nt][8 * w + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+          raw[nt][4 * w + j] = u[j];
+          big = __vmaxu2(big, u[j] & 0x7FFF7FFFu);
+          s[j & 1] = __fadd2_rn(s[j & 1], make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u)));
         }
       }
-      float s = 0.0f, big = 0.0f;
+      s[0] = __fadd2_rn(s[0], s[1]);
+      float total = s[0].x + s[0].y;
+      big = max(big & 0xFFFFu, big >> 16);
 #pragma unroll
-      for (int j = 0; j < W * 8; ++j) {
-        s += q[nt][j];
-        big = fmaxf(big, fabsf(q[nt][j]));
+      for (int d = 1; d < 4; d <<= 1) {
+        total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+        big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
       }
-      s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
-      s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
-      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-      const bool fine = isfinite(s) && isfinite(big);
-      sum[nt] = fine ? s * a.scale2 : __int_as_float(0x7FC00000);
+      const bool fine = big < 0x7F80u;  // no infinity and no NaN in the row
+      sum[nt] = fine ? total * a.scale2 : __int_as_float(0x7FC00000);
       if (fine) {
-        top = fmaxf(top, big);
+        top = max(top, big);
       } else {
 #pragma unroll
-        for (int j = 0; j < W * 8; ++j) q[nt][j] = 0.0f;
+        for (int j = 0; j < W * 4; ++j) raw[nt][j] = 0;
       }
     }
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    const int e = top > 0.0f ? static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127 : 0;
+    for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    const int e = top > 0 ? static_cast<int>(top >> 7) - 127 : 0;
     const int up = max(min(14 - e, 100), -103);  // largest element into [2^14, 2^15)
     const float by = __int_as_float((up + 127) << 23);
     mul = a.scale2 * __int_as_float((127 + 24 - up) << 23);
@@ -128,258 +139,317 @@ struct DecQuery {
       for (int w = 0; w < W; ++w) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float* x = &q[nt][8 * w + 2 * u];
-          f[nt][2 * w + u][0] = half2_bits(x[0] * by, x[4] * by);
-          f[nt][2 * w + u][1] = half2_bits(x[1] * by * 0.0625f, x[5] * by * 0.0625f);
+          // elements 2u, 2u + 1 and 2u + 4, 2u + 5 of eight: the order of the nibbles (0, 4), (1, 5) ... of a word
+          const uint32_t p = raw[nt][4 * w + u], r = raw[nt][4 * w + u + 2];
+          const float2 even = __fmul2_rn(make_float2(__uint_as_float(p << 16), __uint_as_float(r << 16)), both(by));
+          const float2 odd = __fmul2_rn(make_float2(__uint_as_float(p & 0xFFFF0000u), __uint_as_float(r & 0xFFFF0000u)),
+                                        both(by * 0.0625f));
+          f[nt][2 * w + u][0] = half2_bits(even.x, even.y);
+          f[nt][2 * w + u][1] = half2_bits(odd.x, odd.y);
         }
       }
+      zq[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, sum[nt], 8 * t), __shfl_sync(0xFFFFFFFFu, sum[nt], 8 * t + 4));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        zq[nt][i] = __shfl_sync(0xFFFFFFFFu, sum[nt], (2 * t + i) * 4);
         const int r = k.rt * R + nt * 8 + 2 * t + i;
-        pos[nt][i] = r < rows ? k.seq.kv - k.seq.n + r / a.G : -1;
+        pos[nt][i] = r < rows ? k.seq.kv - k.seq.n + a.g.by(r) : -1;
       }
     }
   }
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kDecThreads)
-kv4_decode_kernel(const Kv4AttnArgs a, int* status) {
+__global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2)
+kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
   grid_dep_launch_dependents();
   extern __shared__ __align__(128) uint8_t smem[];
   using L = DecSmem<HD, NT>;
   constexpr int R = L::R, MT = HD / 16, W = HD / 32;
-  __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * kDecStages * L::kStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * kDecStages;
   uint32_t* valid = reinterpret_cast<uint32_t*>(smem + L::kOffValid) + warp * kDecStages;
-  long long* scan = reinterpret_cast<long long*>(smem + L::kOffScan);
-  if (threadIdx.x == 0) s_abort = 0;
-  if (lane == 0) {
-    for (int i = 0; i < kDecStages; ++i) mbar_init(bars + i, 1);
-    fence_mbar_init();
-  }
   grid_dep_wait();
-  const Kv4Share sh = kv4_share<kDecTile, kDecThreads>(a.c, a.m, a.G, R, kDecLeast, scan);
-  const long long begin = blockIdx.x * sh.share;
-  if (begin >= sh.total) return;
-  Kv4Cursor at;
-  kv4_locate<kDecTile, kDecThreads>(a.c, a.m, a.G, R, begin, min(sh.share, sh.total - begin), scan, at);
+  // One warp looks up the CTA's share: its loads go to lines that every CTA wants at once.
+  Kv4Cursor& found = *reinterpret_cast<Kv4Cursor*>(smem + L::kOffCursor);
+  int* s_share = reinterpret_cast<int*>(&found + 1);  // tiles of a CTA; 0: none for this one
+  if (warp == 0) {
+    const Kv4Start k = kv4_begin<kDecTile>(a.c, a.m, a.g, R, kDecLeast, a.grid, lane);
+    if (lane == 0) {
+      if (k.any) found = k.k;
+      else a.join[blockIdx.x].parts = 0;
+      *s_share = k.any ? k.share : 0;
+    }
+  }
+  __syncthreads();
+  const int share = *s_share;
+  if (share == 0) return;
+  Kv4Cursor at = found;
   Kv4Cursor ahead = at;  // where the copies are
   const int P = 1 << a.c.page_shift;
-  const int step = min(P, kDecTile), pieces = kDecTile / step;
-  const uint64_t policy = l2_policy_evict_first();
 
-  // Lane l copies part l % 4 (key codes, value codes, key pairs, value pairs) of page piece l / 4 of a tile.
-  const int piece = lane >> 2, part = lane & 3;
-  const int part_src = part == 0 ? 0 : part == 1 ? P * (HD / 2) : part == 2 ? P * HD : P * HD + 4 * P;
-  const int part_dst = part == 0 ? 0 : part == 1 ? kDecTile * (HD / 2) : part == 2 ? kDecTile * HD : kDecTile * (HD + 4);
-  const int per_token = part < 2 ? HD / 2 : 4;
+  // A tile arrives in pieces of 16 tokens, each of one page: lane l copies every 32nd 16 bytes of the codes, lanes 0 to 7 the
+  // pairs.  The page of piece i is kept by lane i, one tile ahead.
   bool more = true;
-  int next_u = ahead.u0 + warp, next_page = -1, next_slot = 0;
-  // the warp's next tile, and its page
-  auto seek = [&]() {
-    while (more && next_u >= ahead.u1) {
-      more = kv4_next_segment<kDecTile>(a.c, a.m, a.G, R, ahead);
+  int next_u = ahead.u0 + warp, next_page = -1, next_tok = 0;
+  const uint8_t *src_codes = nullptr, *src_pairs = nullptr;  // the lane's 16 bytes of the head's block in page 0
+  const int32_t* table_row = nullptr;                        // the sequence's pages
+  int there = 0;                                             // the sequence's tokens that the table has room for
+  int q_ahead = 0;
+  auto seek_segment = [&]() {
+    const uint8_t* block = a.c.pages + static_cast<int64_t>(ahead.h) * P * (HD + 8);
+    src_codes = block + lane * 16;
+    src_pairs = block + P * HD + ((lane >> 2) & 1) * 4 * P + (lane & 3) * 16;
+    table_row = a.c.table + ahead.b * a.c.table_stride;
+    there = min(ahead.seq.kv, a.c.capacity);
+  };
+  auto copy_queries = [&]() {
+    if (warp == 0) {
+      const int first_row = ahead.rt * R, rows = ahead.seq.n * a.g.G;
+      const uint32_t to = smem_u32(smem + L::kOffQ) + q_ahead * L::kQBytes;
+      for (int c = lane; c < R * HD / 8; c += 32) {
+        const int row = c / (HD / 8), col = c % (HD / 8), r = first_row + row;
+        const bool is = r < rows;
+        const int i = is ? a.g.by(r) : 0, head = ahead.h * a.g.G + (is ? r - i * a.g.G : 0);
+        cp_async_16_or_zero(to + row * kQPitch<HD> + col * 16,
+                            a.q + static_cast<int64_t>(ahead.seq.row0 + i) * a.q_row + static_cast<int64_t>(head) * a.q_head + col * 8,
+                            is);
+      }
+      if (++q_ahead == kDecQueries) q_ahead = 0;
+    }
+  };
+  auto seek = [&]() {  // the warp's next tile, and its pages
+    bool other = false;
+    while (next_u >= ahead.u1) {
+      other = true;
+      more = kv4_next_segment<kDecTile>(a.c, a.m, a.g, R, ahead);
+      if (!more) return;
       next_u = ahead.u0 + warp;
+      seek_segment();
     }
-    next_page = -1;
-    if (more && piece < pieces) {
-      const int tok = ahead.span.tile(next_u) * kDecTile + piece * step;
-      next_slot = tok & (P - 1);
-      if (tok < min(ahead.seq.kv, a.c.capacity)) next_page = a.c.table[ahead.b * a.c.table_stride + (tok >> a.c.page_shift)];
-    }
+    next_tok = ahead.span.tile(next_u) * kDecTile;
+    const int tok = next_tok + lane * 16;
+    next_page = lane < kPieces && tok < there ? table_row[tok >> a.c.page_shift] : -1;
+    if (other) copy_queries();
   };
+  const uint32_t dst_codes = smem_u32(ring) + lane * 16;
+  const uint32_t dst_pairs = smem_u32(ring) + kDecTile * HD + ((lane >> 2) & 1) * kDecTile * 4 + (lane & 3) * 16;
+  const uint32_t page_bytes = static_cast<uint32_t>(a.c.page_stride);
   auto fetch = [&](int stage) {
-    if (!more) return;
-    const bool ok = next_page >= 0 && next_page < a.c.num_pages;
-    const uint32_t got = __ballot_sync(0xFFFFFFFFu, ok) & 0x11111111u;  // one bit per piece
-    if (lane == 0) {
-      valid[stage] = got;
-      mbar_expect_tx(bars + stage, __popc(got) * step * (HD + 8));
+    if (more) {
+      const uint32_t got = __ballot_sync(0xFFFFFFFFu, static_cast<uint32_t>(next_page) < static_cast<uint32_t>(a.c.num_pages));
+      if (lane == 0) valid[stage] = got;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t page = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, next_page, i));
+        if ((got >> i) & 1u) {
+          const uint64_t off = static_cast<uint64_t>(page) * page_bytes;
+          const int slot = (next_tok + 16 * i) & (P - 1);
+          const uint8_t* codes = src_codes + off + slot * (HD / 2);
+          const uint32_t to = dst_codes + stage * L::kStage + i * 16 * (HD / 2);
+#pragma unroll
+          for (int j = 0; j < HD / 64; ++j) {
+            cp_async_16(to + j * 512, codes + j * 512);
+            cp_async_16(to + kDecTile * (HD / 2) + j * 512, codes + P * (HD / 2) + j * 512);
+          }
+          if (lane < 8) cp_async_16(dst_pairs + stage * L::kStage + i * 64, src_pairs + off + slot * 4);
+        }
+      }
+      next_u += kDecWarps;
+      seek();
     }
-    __syncwarp();
-    if (ok) {
-      const uint8_t* src = a.c.pages + next_page * a.c.page_stride + static_cast<int64_t>(ahead.h) * P * (HD + 8) + part_src +
-                           next_slot * per_token;
-      bulk_load_1d(ring + stage * L::kStage + part_dst + piece * step * per_token, src, step * per_token, bars + stage, policy);
-    }
-    next_u += kDecWarps;
-    seek();
+    asm volatile("cp.async.commit_group;" ::: "memory");  // (an empty one too: groups are counted)
   };
+  seek_segment();
   seek();
-  for (int i = 0; i < kDecStages; ++i) fetch(i);
+  copy_queries();
+  asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll 1
+  for (int i = 0; i < kDecStages - 1; ++i) fetch(i);
+  // the first segment's queries have arrived (the others': see kDecQueries)
+  asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 1) : "memory");
+  __syncthreads();
 
-  int stage = 0;
-  uint32_t parity = 0;
-  const uint32_t all_pieces = pieces == 1 ? 0x1u : 0x11u;
-  const int first_b = at.b, first_h = at.h, first_rt = at.rt;
-  for (;;) {
+  int stage = 0, q_at = 0;
+  bool is_first = true, goes_on = false;
+  for (;; is_first = false) {
     DecQuery<HD, NT> q;
-    q.load(a, at, lane);
-    float o[NT][MT][4], m[NT][2], l[NT][2], z[NT][2];
+    q.load(a, at, smem + L::kOffQ + q_at * L::kQBytes, lane);
+    if (++q_at == kDecQueries) q_at = 0;
+    float o[NT][MT][4];
+    float2 m[NT], l[NT], z[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        m[nt][i] = kNoMax;
-        l[nt][i] = z[nt][i] = 0.0f;
-      }
+      m[nt] = make_float2(kNoMax, kNoMax);
+      l[nt] = z[nt] = make_float2(0.0f, 0.0f);
     }
     const int kv = min(at.seq.kv, a.c.capacity);
     for (int u = at.u0 + warp; u < at.u1; u += kDecWarps) {
       const uint8_t* buf = ring + stage * L::kStage;
       const int base = at.span.tile(u) * kDecTile;
-      mbar_wait(bars + stage, parity, &s_abort, 41);
+      fetch(stage == 0 ? kDecStages - 1 : stage - 1);  // into the tile that was read last
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 1) : "memory");
+      __syncwarp();
       const uint32_t got = valid[stage];
       // every row sees every token of the tile?
-      const bool whole = got == all_pieces && base + kDecTile <= kv && base + kDecTile <= at.span.p_lo + 1 &&
+      const bool whole = got == (1u << kPieces) - 1 && base + kDecTile <= kv && base + kDecTile <= at.span.p_lo + 1 &&
                          (a.m.window == 0 || base > at.span.p_hi - a.m.window || base + kDecTile <= a.m.sinks);
       const __half2* kpar = reinterpret_cast<const __half2*>(buf + kDecTile * HD);
       const __half2* vpar = kpar + kDecTile;
+      // S' = K Q': rows g and g + 8 are tokens.  Two chains of sums for each 16 tokens: a chain's products wait for one another
+      float2 x[kPieces][NT][2];  // scores of tokens 16 i + g and 16 i + g + 8, query rows 2t and 2t + 1
 #pragma unroll
-      for (int half = 0; half < kDecTile / 16; ++half) {
-        float s[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-        // S' = K Q': rows g and g + 8 are tokens
-        {
-          uint32_t ka[W], kb[W];
-          const uint8_t* row = buf + (half * 16 + g) * (HD / 2) + t * (HD / 8);
-          if constexpr (W == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(row), y = *reinterpret_cast<const uint4*>(row + 8 * (HD / 2));
-            ka[0] = x.x, ka[1] = x.y, ka[2] = x.z, ka[3] = x.w;
-            kb[0] = y.x, kb[1] = y.y, kb[2] = y.z, kb[3] = y.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(row), y = *reinterpret_cast<const uint2*>(row + 8 * (HD / 2));
-            ka[0] = x.x, ka[1] = x.y;
-            kb[0] = y.x, kb[1] = y.y;
-          }
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              const uint32_t xa = ka[w] >> (8 * v), xb = kb[w] >> (8 * v);
-              const uint32_t a0 = xa & 0x000F000Fu, a1 = xb & 0x000F000Fu, a2 = xa & 0x00F000F0u, a3 = xb & 0x00F000F0u;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, q.f[nt][2 * w + v][0], q.f[nt][2 * w + v][1]);
-            }
+      for (int i = 0; i < kPieces; ++i) {
+        uint32_t ka[W], kb[W];
+        const uint8_t* row = buf + (i * 16 + g) * (HD / 2) + t * (HD / 8);
+        if constexpr (W == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(row), v = *reinterpret_cast<const uint4*>(row + 8 * (HD / 2));
+          ka[0] = u.x, ka[1] = u.y, ka[2] = u.z, ka[3] = u.w;
+          kb[0] = v.x, kb[1] = v.y, kb[2] = v.z, kb[3] = v.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(row), v = *reinterpret_cast<const uint2*>(row + 8 * (HD / 2));
+          ka[0] = u.x, ka[1] = u.y;
+          kb[0] = v.x, kb[1] = v.y;
         }
-        // scores, weights
-        const int key = half * 16 + g;
-        const float2 k0 = __half22float2(kpar[key]), k1 = __half22float2(kpar[key + 8]);
-        __half2 v0h = vpar[key], v1h = vpar[key + 8];
-        if (!whole) {  // slots that hold no token may hold anything
-          if (base + key >= kv) v0h = __half2half2(__ushort_as_half(0));
-          if (base + key + 8 >= kv) v1h = __half2half2(__ushort_as_half(0));
-        }
-        const float2 v0 = __half22float2(v0h), v1 = __half22float2(v1h);
-        const float e0 = static_cast<float>(static_cast<int>((__half_as_ushort(__low2half(v0h)) >> 10) & 31u) - 15);
-        const float e1 = static_cast<float>(static_cast<int>((__half_as_ushort(__low2half(v1h)) >> 10) & 31u) - 15);
-        const float s0 = k0.x * q.mul, s1 = k1.x * q.mul;
-        bool lift = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            s[nt][i] = fmaf(s0, s[nt][i], k0.y * q.zq[nt][i]);
-            s[nt][2 + i] = fmaf(s1, s[nt][2 + i], k1.y * q.zq[nt][i]);
-          }
-        }
-        if (!whole) {
-          const bool here0 = (got >> (4 * (key / step))) & 1u, here1 = (got >> (4 * ((key + 8) / step))) & 1u;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int p = q.pos[nt][i], j0 = base + key, j1 = j0 + 8;
-              const bool see0 = here0 && j0 < kv && j0 <= p && (a.m.window == 0 || j0 > p - a.m.window || j0 < a.m.sinks);
-              const bool see1 = here1 && j1 < kv && j1 <= p && (a.m.window == 0 || j1 > p - a.m.window || j1 < a.m.sinks);
-              if (!see0) s[nt][i] = -INFINITY;
-              if (!see1) s[nt][2 + i] = -INFINITY;
-            }
-        }
+        float s[NT][2][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            lift |= fmaxf(s[nt][i] + e0, s[nt][2 + i] + e1) > m[nt][i] + 8.0f;
-        if (__any_sync(0xFFFFFFFFu, lift)) {
+          for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.0f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int w = 0; w < W; ++w)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float top = fmaxf(s[nt][i] + e0, s[nt][2 + i] + e1);
+          for (int v = 0; v < 2; ++v) {
+            const uint32_t xa = ka[w] >> (8 * v), xb = kb[w] >> (8 * v);
+            const uint32_t a0 = xa & 0x000F000Fu, a1 = xb & 0x000F000Fu, a2 = xa & 0x00F000F0u, a3 = xb & 0x00F000F0u;
 #pragma unroll
-              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-              top = fmaxf(top, m[nt][i]);
-              const float by = exp2_approx(m[nt][i] - top);
-              m[nt][i] = top;
-              l[nt][i] *= by;
-              z[nt][i] *= by;
-#pragma unroll
-              for (int j = 0; j < MT; ++j) {
-                o[nt][j][i] *= by;
-                o[nt][j][2 + i] *= by;
-              }
-            }
-        }
-        uint32_t pb[NT][2];
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt][v], a0, a1, a2, a3, q.f[nt][2 * w + v][0], q.f[nt][2 * w + v][1]);
+          }
+        const float2 k0 = __half22float2(kpar[i * 16 + g]), k1 = __half22float2(kpar[i * 16 + g + 8]);
+        const float2 s0 = both(k0.x * q.mul), s1 = both(k1.x * q.mul);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float w0[2], w1[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float p0 = exp2_approx(s[nt][i] - m[nt][i]), p1 = exp2_approx(s[nt][2 + i] - m[nt][i]);
-            l[nt][i] += p0 + p1;
-            z[nt][i] = fmaf(p0, v0.y, fmaf(p1, v1.y, z[nt][i]));
-            w0[i] = p0 * v0.x;
-            w1[i] = p1 * v1.x;
-          }
-          pb[nt][0] = transpose_8x8(half2_bits(w0[0], w0[1]));
-          pb[nt][1] = transpose_8x8(half2_bits(w1[0], w1[1]));
+          x[i][nt][0] = __ffma2_rn(s0, __fadd2_rn(make_float2(s[nt][0][0], s[nt][0][1]), make_float2(s[nt][1][0], s[nt][1][1])),
+                                   __fmul2_rn(both(k0.y), q.zq[nt]));
+          x[i][nt][1] = __ffma2_rn(s1, __fadd2_rn(make_float2(s[nt][0][2], s[nt][0][3]), make_float2(s[nt][1][2], s[nt][1][3])),
+                                   __fmul2_rn(both(k1.y), q.zq[nt]));
         }
-        // O' += V' P': rows g and g + 8 are head elements, columns of V' the tokens 2t, 2t + 1, 2t + 8, 2t + 9
-        {
-          constexpr int VW = HD / 64;  // words of a token's value codes per lane
-          const uint8_t* row = buf + kDecTile * (HD / 2) + (half * 16 + 2 * t) * (HD / 2) + g * (HD / 16);
-          uint32_t v[4][VW];
+      }
+      // value scales and zeros, and the exponents of the scales
+      float2 vp[kPieces][2];
+      float ve[kPieces][2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint8_t* p = row + ((i & 1) + 8 * (i >> 1)) * (HD / 2);
-            if constexpr (VW == 2) {
-              const uint2 x = *reinterpret_cast<const uint2*>(p);
-              v[i][0] = x.x, v[i][1] = x.y;
-            } else {
-              v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          __half2 h = vpar[i * 16 + 8 * j + g];
+          // slots that hold no token may hold anything
+          if (!whole && (base + i * 16 + 8 * j + g >= kv || !((got >> i) & 1u))) h = __half2half2(__ushort_as_half(0));
+          vp[i][j] = __half22float2(h);
+          ve[i][j] = static_cast<float>(static_cast<int>((__half_as_ushort(__low2half(h)) >> 10) & 31u) - 15);
+        }
+      if (!whole) {
+        auto see = [&](int i, int j, int p) {
+          return ((got >> i) & 1u) && j < kv && j <= p && (a.m.window == 0 || j > p - a.m.window || j < a.m.sinks);
+        };
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int tok = base + i * 16 + 8 * j + g;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (!see(i, tok, q.pos[nt][0])) x[i][nt][j].x = -INFINITY;
+              if (!see(i, tok, q.pos[nt][1])) x[i][nt][j].y = -INFINITY;
             }
           }
+      }
+      bool lift = false;
+      float2 high[NT];
 #pragma unroll
-          for (int w = 0; w < VW; ++w)
+      for (int nt = 0; nt < NT; ++nt) {
+        high[nt] = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
-              const uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
+        for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const uint32_t xs = x >> (8 * c), ys = y >> (8 * c);
-                const uint32_t a0 = xs & 0x000F000Fu, a1 = xs & 0x00F000F0u, a2 = ys & 0x000F000Fu, a3 = ys & 0x00F000F0u;
+          for (int j = 0; j < 2; ++j) {
+            const float2 v = __fadd2_rn(x[i][nt][j], both(ve[i][j]));
+            high[nt] = make_float2(fmaxf(high[nt].x, v.x), fmaxf(high[nt].y, v.y));
+          }
+        lift |= high[nt].x > m[nt].x + 8.0f || high[nt].y > m[nt].y + 8.0f;
+      }
+      if (__any_sync(0xFFFFFFFFu, lift)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][(w * 2 + h) * 2 + c], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-              }
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            high[nt].x = fmaxf(high[nt].x, __shfl_xor_sync(0xFFFFFFFFu, high[nt].x, d));
+            high[nt].y = fmaxf(high[nt].y, __shfl_xor_sync(0xFFFFFFFFu, high[nt].y, d));
+          }
+          high[nt] = make_float2(fmaxf(high[nt].x, m[nt].x), fmaxf(high[nt].y, m[nt].y));
+          const float2 by = make_float2(exp2_approx(m[nt].x - high[nt].x), exp2_approx(m[nt].y - high[nt].y));
+          m[nt] = high[nt];
+          l[nt] = __fmul2_rn(l[nt], by);
+          z[nt] = __fmul2_rn(z[nt], by);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            o[nt][j][0] *= by.x, o[nt][j][1] *= by.y;
+            o[nt][j][2] *= by.x, o[nt][j][3] *= by.y;
+          }
         }
+      }
+      // weights
+      uint32_t pb[kPieces][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 low = make_float2(-m[nt].x, -m[nt].y);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 y = __fadd2_rn(x[i][nt][j], low);
+            const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            l[nt] = __fadd2_rn(l[nt], p);
+            z[nt] = __ffma2_rn(p, both(vp[i][j].y), z[nt]);
+            const float2 w = __fmul2_rn(p, both(vp[i][j].x));
+            pb[i][nt][j] = transpose_8x8(half2_bits(w.x, w.y));
+          }
+      }
+      // O' += V' P': rows g and g + 8 are head elements, columns of V' the tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        constexpr int VW = HD / 64;  // words of a token's value codes per lane
+        const uint8_t* row = buf + kDecTile * (HD / 2) + (i * 16 + 2 * t) * (HD / 2) + g * (HD / 16);
+        uint32_t v[4][VW];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint8_t* p = row + ((c & 1) + 8 * (c >> 1)) * (HD / 2);
+          if constexpr (VW == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            v[c][0] = u.x, v[c][1] = u.y;
+          } else {
+            v[c][0] = *reinterpret_cast<const uint32_t*>(p);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
+            const uint32_t hi = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t ls = lo >> (8 * c), hs = hi >> (8 * c);
+              const uint32_t a0 = ls & 0x000F000Fu, a1 = ls & 0x00F000F0u, a2 = hs & 0x000F000Fu, a3 = hs & 0x00F000F0u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16(o[nt][(w * 2 + h) * 2 + c], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+            }
+          }
       }
       __syncwarp();  // every lane has read the tile
-      fetch(stage);
-      if (++stage == kDecStages) {
-        stage = 0;
-        parity ^= 1;
-      }
+      if (++stage == kDecStages) stage = 0;
     }
     // the warps' sums meet
     float* meet = reinterpret_cast<float*>(smem + L::kOffMeet);
@@ -388,27 +458,39 @@ kv4_decode_kernel(const Kv4AttnArgs a, int* status) {
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        float ls = i ? l[nt].y : l[nt].x, zs = i ? z[nt].y : z[nt].x;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
-          l[nt][i] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][i], d);
-          z[nt][i] += __shfl_xor_sync(0xFFFFFFFFu, z[nt][i], d);
+          ls += __shfl_xor_sync(0xFFFFFFFFu, ls, d);
+          zs += __shfl_xor_sync(0xFFFFFFFFu, zs, d);
         }
         const int r = nt * 8 + 2 * t + i;
         float* dst = meet + (warp * R + r) * L::kPitch + g * (2 * MT);
 #pragma unroll
         for (int j = 0; j < MT / 2; ++j)
           reinterpret_cast<float4*>(dst)[j] =
-              make_float4(fmaf(o[nt][2 * j][i], 16777216.0f, z[nt][i]), fmaf(o[nt][2 * j][2 + i], 1048576.0f, z[nt][i]),
-                          fmaf(o[nt][2 * j + 1][i], 16777216.0f, z[nt][i]), fmaf(o[nt][2 * j + 1][2 + i], 1048576.0f, z[nt][i]));
+              make_float4(fmaf(o[nt][2 * j][i], 16777216.0f, zs), fmaf(o[nt][2 * j][2 + i], 1048576.0f, zs),
+                          fmaf(o[nt][2 * j + 1][i], 16777216.0f, zs), fmaf(o[nt][2 * j + 1][2 + i], 1048576.0f, zs));
         if (g == 0) {
-          ml[(warp * R + r) * 2] = m[nt][i];
-          ml[(warp * R + r) * 2 + 1] = l[nt][i];
+          ml[(warp * R + r) * 2] = i ? m[nt].y : m[nt].x;
+          ml[(warp * R + r) * 2 + 1] = ls;
         }
       }
     __syncthreads();
-    const int rows = min(R, at.seq.n * a.G - at.rt * R);
+    const int rows = min(R, at.seq.n * a.g.G - at.rt * R);
     const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
-    const bool is_first = at.b == first_b && at.h == first_h && at.rt == first_rt;
+    if (at.u0 == 0 && at.u1 < at.span.count && threadIdx.x == 0) {
+      // (the segment reaches the end of this CTA's share, and share tiles a CTA from there on)
+      Kv4Join j;
+      j.parts = 1 + (at.span.count - at.u1 + share - 1) / share;
+      j.slot = is_first ? 0 : 1;
+      j.rows = rows;
+      j.first_row = at.rt * R;
+      j.row0 = at.seq.row0;
+      j.h = at.h;
+      a.join[blockIdx.x] = j;
+    }
+    goes_on |= at.u0 == 0 && at.u1 < at.span.count;
     float* part_out = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(R, HD);
     for (int r = threadIdx.x / HD; r < rows; r += kDecThreads / HD) {
       const int d = threadIdx.x % HD;
@@ -422,12 +504,12 @@ kv4_decode_kernel(const Kv4AttnArgs a, int* status) {
         acc = fmaf(by, meet[(w * R + r) * L::kPitch + d], acc);
       }
       if (whole_segment) {
-        const int at_row = at.rt * R + r, i = at_row / a.G, head = at.h * a.G + (at_row - i * a.G);
+        const int at_row = at.rt * R + r, i = a.g.by(at_row), head = at.h * a.g.G + (at_row - i * a.g.G);
         // no token seen: zero (and not 0 / 0); a row that is not finite stays NaN
         const float val = sum == 0.0f ? 0.0f : __fdividef(acc, sum);
         unsigned short bits;
         asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(bits) : "f"(val));
-        a.out[(static_cast<int64_t>(at.seq.row0 + i) * a.c.hkv * a.G + head) * HD + d] = bits;
+        a.out[(static_cast<int64_t>(at.seq.row0 + i) * a.c.hkv * a.g.G + head) * HD + d] = bits;
       } else {
         part_out[2 * R + r * HD + d] = acc;
         if (d == 0) {
@@ -436,50 +518,71 @@ kv4_decode_kernel(const Kv4AttnArgs a, int* status) {
         }
       }
     }
-    if (!kv4_next_segment<kDecTile>(a.c, a.m, a.G, R, at)) break;
+    if (!kv4_next_segment<kDecTile>(a.c, a.m, a.g, R, at)) break;
     __syncthreads();
   }
-  __syncthreads();
-  if (threadIdx.x == 0 && s_abort != 0) atomicExch(status, s_abort);
+  if (threadIdx.x == 0 && !goes_on) a.join[blockIdx.x].parts = 0;
 }
 
-// Joins what several CTAs hold of a segment: block c the segment that begins in CTA c of the kernel before it and goes on
-// behind it.  Always the same sums in the same order.
-template <int HD, int R, int TK, int LEAST>
+// Joins what several CTAs hold of a segment: block (c, y) the rows y, y + gridDim.y ... of the segment that begins in CTA c of
+// the kernel before it and goes on behind it.  A lane holds HD / 32 elements of a row, the warps take every eighth part and
+// meet in shared memory: always the same sums in the same order.
+template <int HD, int R>
 __global__ void __launch_bounds__(256)
 kv4_combine_kernel(const Kv4AttnArgs a) {
   grid_dep_launch_dependents();
-  __shared__ long long scan[257];
+  constexpr int E = HD / 32;
+  __shared__ float s_acc[8][HD], s_l[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dep_wait();
-  const Kv4Share sh = kv4_share<TK, 256>(a.c, a.m, a.G, R, LEAST, scan);
-  const long long begin = blockIdx.x * sh.share, end = begin + sh.share;
-  if (end >= sh.total) return;  // the last CTA's segments end with it
-  Kv4Cursor k;
-  const long long first = kv4_locate<TK, 256>(a.c, a.m, a.G, R, end - 1, 1, scan, k);
-  const long long last = first + k.span.count - 1;
-  if (first < begin || last < end) return;
-  const int parts = static_cast<int>(last / sh.share - blockIdx.x) + 1;
-  const int rows = min(R, k.seq.n * a.G - k.rt * R);
-  const int d = threadIdx.x % HD;
-  for (int r = threadIdx.x / HD + (256 / HD) * blockIdx.y; r < rows; r += (256 / HD) * gridDim.y) {
-    float top = kNoMax, sum = 0.0f, acc = 0.0f;
-    auto at = [&](int p) {
-      const size_t slot = static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 && first > begin ? 1 : 0);
-      return a.partial + slot * kv4_partial_floats(R, HD);
-    };
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, at(p)[2 * r]);
+  const Kv4Join j = a.join[blockIdx.x];
+  if (j.parts == 0) return;
+  auto part = [&](int p) {
+    return a.partial + (static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 ? j.slot : 0)) * kv4_partial_floats(R, HD);
+  };
+  for (int r = blockIdx.y; r < j.rows; r += gridDim.y) {
+    float top = kNoMax;
+    for (int p = lane; p < j.parts; p += 32) top = fmaxf(top, part(p)[2 * r]);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    float sum = 0.0f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
 #pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      const float* s = at(p);
+    for (int p = warp; p < j.parts; p += 8) {
+      const float* s = part(p);
       const float by = exp2_approx(s[2 * r] - top);
       sum = fmaf(by, s[2 * r + 1], sum);
-      acc = fmaf(by, s[2 * R + r * HD + d], acc);
+      const float* o = s + 2 * R + r * HD + lane * E;
+      float v[E];
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(o);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(o);
+        v[0] = x.x, v[1] = x.y;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(by, v[e], acc[e]);
     }
-    const int at_row = k.rt * R + r, i = at_row / a.G, head = k.h * a.G + (at_row - i * a.G);
-    const float val = sum == 0.0f ? 0.0f : __fdividef(acc, sum);
-    unsigned short bits;
-    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(bits) : "f"(val));
-    a.out[(static_cast<int64_t>(k.seq.row0 + i) * a.c.hkv * a.G + head) * HD + d] = bits;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
+    if (lane == 0) s_l[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x < HD) {
+      float l = 0.0f, o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        l += s_l[w];
+        o += s_acc[w][threadIdx.x];
+      }
+      const int at_row = j.first_row + r, i = a.g.by(at_row), head = j.h * a.g.G + (at_row - i * a.g.G);
+      const float val = l == 0.0f ? 0.0f : __fdividef(o, l);
+      unsigned short bits;
+      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(bits) : "f"(val));
+      a.out[(static_cast<int64_t>(j.row0 + i) * a.c.hkv * a.g.G + head) * HD + threadIdx.x] = bits;
+    }
+    __syncthreads();
   }
 }
 
@@ -504,20 +607,21 @@ int init_kv4_decode_kernels() {
 }
 
 template <int HD, int NT>
-static int launch_decode(const Kv4AttnArgs& a, int grid, cudaStream_t s, DeviceState* st) {
+static int launch_decode(const Kv4AttnArgs& a, int grid, cudaStream_t s) {
   constexpr int R = 8 * NT;
-  DQ_CHECK_CUDA(launch_pdl(kv4_decode_kernel<HD, NT>, dim3(grid), dim3(kDecThreads), DecSmem<HD, NT>::kBytes, s, a,
-                           st->status_dev));
+  DQ_CHECK_CUDA(launch_pdl(kv4_decode_kernel<HD, NT>, dim3(grid), dim3(kDecThreads), DecSmem<HD, NT>::kBytes, s, a));
   if (grid > 1)
-    DQ_CHECK_CUDA(launch_pdl(kv4_combine_kernel<HD, R, kDecTile, kDecLeast>, dim3(grid, R * HD / 256 > 4 ? 4 : R * HD / 256), dim3(256), 0, s, a));
+    DQ_CHECK_CUDA(launch_pdl(kv4_combine_kernel<HD, R>, dim3(grid, R < 4 ? R : 4), dim3(256), 0, s, a));
   return DQ_OK;
 }
 
-// Grid of a call: enough CTAs to fill the GPU, and no more than there can be shares.
+// Grid of a call: enough CTAs to fill the GPU, and no more than there can be shares.  0: too many tiles to number.
 static int decode_grid(const Kv4Batch& c, int G, int hd, int R, DeviceState* st) {
   const int64_t row_tiles = (static_cast<int64_t>(c.T) * G + R - 1) / R + c.B;
   const int64_t tiles = (c.capacity + kDecTile - 1) / kDecTile + 1;
-  const int64_t most = (row_tiles * c.hkv * tiles + kDecLeast - 1) / kDecLeast;
+  const int64_t units = row_tiles * c.hkv * tiles;
+  if (units >= (1ll << 31)) return 0;
+  const int64_t most = (units + kDecLeast - 1) / kDecLeast;
   const int64_t fill = static_cast<int64_t>(st->sm_count) * g_resident[hd == 128][R / 8 - 1];
   return static_cast<int>(most < fill ? most : fill);
 }
@@ -534,7 +638,8 @@ extern "C" size_t dq_kv4_attention_workspace_bytes(const dq_kv4_batch* batch, in
   if (st == nullptr || kv4_batch_of(batch, &c) != DQ_OK || hq < 1 || max_new < 1) return 0;
   if (c.B == 0 || c.T == 0) return 0;
   const int G = hq / c.hkv > 0 ? hq / c.hkv : 1, R = kv4_rows(G, max_new);
-  return static_cast<size_t>(decode_grid(c, G, batch->head_dim, R, st)) * 2 * kv4_partial_floats(R, batch->head_dim) * 4;
+  const int grid = decode_grid(c, G, batch->head_dim, R, st);
+  return kv4_join_bytes(grid) + static_cast<size_t>(grid) * 2 * kv4_partial_floats(R, batch->head_dim) * 4;
 }
 
 extern "C" int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, int64_t q_row_stride, int64_t q_head_stride,
@@ -562,12 +667,17 @@ extern "C" int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, i
   a.q_row = q_row_stride;
   a.q_head = q_head_stride;
   a.out = static_cast<unsigned short*>(out_bf16);
-  a.partial = static_cast<float*>(workspace);
-  a.G = hq / a.c.hkv;
+  a.g.G = hq / a.c.hkv;
+  a.g.by = kv4_div(a.g.G);
   a.scale2 = scale * 1.4426950408889634f;
-  const int R = kv4_rows(a.G, max_new), hd = batch->head_dim;
-  const int grid = decode_grid(a.c, a.G, hd, R, st);
+  const int R = kv4_rows(a.g.G, max_new), hd = batch->head_dim;
+  const int grid = decode_grid(a.c, a.g.G, hd, R, st);
+  DQ_REQUIRE(grid > 0, DQ_ERR_SHAPE, "%d rows over %d sequences of up to %d tokens are too many for one call", a.c.T, a.c.B,
+             a.c.capacity);
+  a.grid = kv4_div(grid);
+  a.join = static_cast<Kv4Join*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kv4_join_bytes(grid));
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (hd == 128) return R == 8 ? launch_decode<128, 1>(a, grid, cs, st) : launch_decode<128, 2>(a, grid, cs, st);
-  return R == 8 ? launch_decode<64, 1>(a, grid, cs, st) : launch_decode<64, 2>(a, grid, cs, st);
+  if (hd == 128) return R == 8 ? launch_decode<128, 1>(a, grid, cs) : launch_decode<128, 2>(a, grid, cs);
+  return R == 8 ? launch_decode<64, 1>(a, grid, cs) : launch_decode<64, 2>(a, grid, cs);
 }

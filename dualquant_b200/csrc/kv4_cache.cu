@@ -203,8 +203,8 @@ int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out) {
   DQ_REQUIRE((1 << shift) == in->page_size, DQ_ERR_UNSUPPORTED, "page_size %d: a power of two from 16 to 256", in->page_size);
   const int64_t block = static_cast<int64_t>(in->page_size) * (in->head_dim + 8);
   DQ_REQUIRE(in->num_pages >= 0 && in->num_pages < (1ll << 31), DQ_ERR_SHAPE, "num_pages=%lld", (long long)in->num_pages);
-  DQ_REQUIRE(in->page_stride >= block * in->hkv && in->page_stride % 16 == 0, DQ_ERR_ALIGN,
-             "page_stride %lld: a multiple of 16 and at least hkv blocks of %lld", (long long)in->page_stride, (long long)block);
+  DQ_REQUIRE(in->page_stride >= block * in->hkv && in->page_stride % 16 == 0 && in->page_stride < (1ll << 32), DQ_ERR_ALIGN,
+             "page_stride %lld: a multiple of 16 below 4 GiB and at least hkv blocks of %lld", (long long)in->page_stride, (long long)block);
   DQ_REQUIRE(in->pages_per_seq >= 0 && static_cast<int64_t>(in->pages_per_seq) * in->page_size < (1ll << 30) &&
                  in->table_stride >= in->pages_per_seq,
              DQ_ERR_SHAPE, "pages_per_seq=%d table_stride=%lld", in->pages_per_seq, (long long)in->table_stride);
