@@ -41,7 +41,9 @@ SOURCES = [
     "gemm_fp4_persist.cu",
     "exchange.cu",
     "kv4_cache.cu",
+    "kv4_attn.cu",
     "kv4_attn_decode.cu",
+    "kv4_attn_prefill.cu",
 ]
 
 NVCC_FLAGS = [

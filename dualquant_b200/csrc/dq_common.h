@@ -128,6 +128,7 @@ int init_gemm_a16w4_kernels();
 int init_gemm_int4_f8_kernels();
 int init_gemm_fp4_persist_kernels();
 int init_kv4_decode_kernels();
+int init_kv4_prefill_kernels();
 int launch_gemm_fp4_persist(const uint8_t* x_codes, const uint8_t* x_sf_atoms, const float* x_scale,
                             const uint8_t* w_codes, const uint8_t* w_sf_atoms, const float* w_scale, const float* r,
                             const void* bias, int M, int N, int K, int nvfp4, void* y, int y_dtype, cudaStream_t stream,

@@ -193,6 +193,8 @@ extern "C" int dq_init(int device) {
   if (rc != DQ_OK) return rc;
   rc = init_kv4_decode_kernels();
   if (rc != DQ_OK) return rc;
+  rc = init_kv4_prefill_kernels();
+  if (rc != DQ_OK) return rc;
   DQ_CHECK_CUDA(cudaDeviceSynchronize());
   st->ready = true;
   return DQ_OK;

@@ -195,8 +195,8 @@ __device__ __forceinline__ int kv4_head_of(int in, int per_head) {
 // Any batch: a lane adds up B / 32 neighbouring sequences, and the sequences of the lane that holds the first tile are added up
 // once more, one a lane (two rounds of loads for up to 1024).
 template <int TK>
-__device__ __noinline__ Kv4Start kv4_begin_any(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, int least,
-                                               Kv4Div grid, int lane) {
+__device__ __forceinline__ Kv4Start kv4_begin_any(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, int least,
+                                                  Kv4Div grid, int lane) {
   Kv4Start r;
   Kv4Cursor& k = r.k;
   const int each = (c.B + 31) / 32;
@@ -252,6 +252,12 @@ __device__ __noinline__ Kv4Start kv4_begin_any(const Kv4Batch& c, const Kv4Mask&
 }
 
 template <int TK>
+__device__ __noinline__ Kv4Start kv4_begin_apart(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, int least,
+                                                 Kv4Div grid, int lane) {
+  return kv4_begin_any<TK>(c, m, g, R, least, grid, lane);
+}
+
+template <int TK>
 __device__ __forceinline__ Kv4Start kv4_begin(const Kv4Batch& c, const Kv4Mask& m, const Kv4Group& g, int R, int least, Kv4Div grid,
                                               int lane) {
   constexpr int N = 4;  // sequences of a lane
@@ -265,7 +271,7 @@ __device__ __forceinline__ Kv4Start kv4_begin(const Kv4Batch& c, const Kv4Mask& 
     if (i < each && b < c.B) seq[i] = kv4_seq(c, b);
     one &= seq[i].n * g.G <= R;
   }
-  if (!__all_sync(0xFFFFFFFFu, one)) return kv4_begin_any<TK>(c, m, g, R, least, grid, lane);
+  if (!__all_sync(0xFFFFFFFFu, one)) return kv4_begin_apart<TK>(c, m, g, R, least, grid, lane);
   Kv4Start r;
   int upto[N], n = 0;
 #pragma unroll
@@ -314,7 +320,11 @@ struct Kv4Join {
   int rows, first_row, row0, h;
 };
 __host__ __device__ constexpr size_t kv4_partial_floats(int R, int hd) { return static_cast<size_t>(R) * (hd + 2); }
-__host__ __device__ constexpr size_t kv4_join_bytes(int grid) { return (static_cast<size_t>(grid) * sizeof(Kv4Join) + 255) / 256 * 256; }
+
+// Tiles of the two attention kernels: tokens, query rows, and the least tiles of a CTA.
+constexpr int kDecTile = 32, kDecLeast = 4;                    // 8 or 16 rows
+constexpr int kPreTile = 128, kPreRows = 256, kPreLeast = 2;
+constexpr float kKv4NoMax = -1e30f;  // reference point of a row that has seen no token
 
 int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out);
 
@@ -330,5 +340,9 @@ struct Kv4AttnArgs {
   Kv4Div grid;              // by the number of CTAs
   float scale2;             // softmax scale * log2(e)
 };
+
+int kv4_decode_resident(int hd, int R);  // CTAs per SM
+int launch_kv4_decode(const Kv4AttnArgs& a, int hd, int R, int grid, cudaStream_t s);
+int launch_kv4_prefill(const Kv4AttnArgs& a, int hd, int grid, cudaStream_t s, DeviceState* st);
 
 }  // namespace dq

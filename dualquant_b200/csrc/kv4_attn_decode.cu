@@ -1,5 +1,4 @@
-// Attention of a few query rows per sequence over the paged 4-bit cache (decode steps, drafted tokens), and the kernel that
-// joins the sums of segments which several CTAs share.
+// Attention of a few query rows per sequence over the paged 4-bit cache (decode steps, drafted tokens).
 //
 //   o = sum_j p_j (s_j c_j + z_j) / sum_j p_j,   p_j = 2^(x_j - m),   x_j = scale log2(e) q . (s'_j c'_j + z'_j)
 // with the scales outside of the matrix products:
@@ -23,14 +22,11 @@
 
 namespace dq {
 
-constexpr int kDecTile = 32;     // tokens per tile
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecStages = 2;    // tiles of a warp's ring
 constexpr int kPieces = kDecTile / 16;
 constexpr int kDecQueries = kDecStages + 1;  // query rows of a segment are copied when its predecessor's last tile is
-constexpr int kDecLeast = 4;     // tiles that a CTA takes at least
-constexpr float kNoMax = -1e30f;
 
 template <int HD>
 constexpr int kQPitch = 2 * HD + 16;  // bytes
@@ -281,7 +277,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.0f;
-      m[nt] = make_float2(kNoMax, kNoMax);
+      m[nt] = make_float2(kKv4NoMax, kKv4NoMax);
       l[nt] = z[nt] = make_float2(0.0f, 0.0f);
     }
     const int kv = min(at.seq.kv, a.c.capacity);
@@ -494,7 +490,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     float* part_out = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(R, HD);
     for (int r = threadIdx.x / HD; r < rows; r += kDecThreads / HD) {
       const int d = threadIdx.x % HD;
-      float top = kNoMax, sum = 0.0f, acc = 0.0f;
+      float top = kKv4NoMax, sum = 0.0f, acc = 0.0f;
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, ml[(w * R + r) * 2]);
 #pragma unroll
@@ -524,68 +520,6 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
   if (threadIdx.x == 0 && !goes_on) a.join[blockIdx.x].parts = 0;
 }
 
-// Joins what several CTAs hold of a segment: block (c, y) the rows y, y + gridDim.y ... of the segment that begins in CTA c of
-// the kernel before it and goes on behind it.  A lane holds HD / 32 elements of a row, the warps take every eighth part and
-// meet in shared memory: always the same sums in the same order.
-template <int HD, int R>
-__global__ void __launch_bounds__(256)
-kv4_combine_kernel(const Kv4AttnArgs a) {
-  grid_dep_launch_dependents();
-  constexpr int E = HD / 32;
-  __shared__ float s_acc[8][HD], s_l[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_dep_wait();
-  const Kv4Join j = a.join[blockIdx.x];
-  if (j.parts == 0) return;
-  auto part = [&](int p) {
-    return a.partial + (static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 ? j.slot : 0)) * kv4_partial_floats(R, HD);
-  };
-  for (int r = blockIdx.y; r < j.rows; r += gridDim.y) {
-    float top = kNoMax;
-    for (int p = lane; p < j.parts; p += 32) top = fmaxf(top, part(p)[2 * r]);
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    float sum = 0.0f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-    for (int p = warp; p < j.parts; p += 8) {
-      const float* s = part(p);
-      const float by = exp2_approx(s[2 * r] - top);
-      sum = fmaf(by, s[2 * r + 1], sum);
-      const float* o = s + 2 * R + r * HD + lane * E;
-      float v[E];
-      if constexpr (E == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(o);
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(o);
-        v[0] = x.x, v[1] = x.y;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(by, v[e], acc[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
-    if (lane == 0) s_l[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x < HD) {
-      float l = 0.0f, o = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        l += s_l[w];
-        o += s_acc[w][threadIdx.x];
-      }
-      const int at_row = j.first_row + r, i = a.g.by(at_row), head = j.h * a.g.G + (at_row - i * a.g.G);
-      const float val = l == 0.0f ? 0.0f : __fdividef(o, l);
-      unsigned short bits;
-      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(bits) : "f"(val));
-      a.out[(static_cast<int64_t>(j.row0 + i) * a.c.hkv * a.g.G + head) * HD + threadIdx.x] = bits;
-    }
-    __syncthreads();
-  }
-}
-
 static int g_resident[2][2];  // CTAs per SM of kv4_decode_kernel<64 or 128, 1 or 2>
 
 template <int HD, int NT>
@@ -606,78 +540,16 @@ int init_kv4_decode_kernels() {
   return rc;
 }
 
+int kv4_decode_resident(int hd, int R) { return g_resident[hd == 128][R / 8 - 1]; }
+
 template <int HD, int NT>
 static int launch_decode(const Kv4AttnArgs& a, int grid, cudaStream_t s) {
-  constexpr int R = 8 * NT;
   DQ_CHECK_CUDA(launch_pdl(kv4_decode_kernel<HD, NT>, dim3(grid), dim3(kDecThreads), DecSmem<HD, NT>::kBytes, s, a));
-  if (grid > 1)
-    DQ_CHECK_CUDA(launch_pdl(kv4_combine_kernel<HD, R>, dim3(grid, R < 4 ? R : 4), dim3(256), 0, s, a));
   return DQ_OK;
 }
-
-// Grid of a call: enough CTAs to fill the GPU, and no more than there can be shares.  0: too many tiles to number.
-static int decode_grid(const Kv4Batch& c, int G, int hd, int R, DeviceState* st) {
-  const int64_t row_tiles = (static_cast<int64_t>(c.T) * G + R - 1) / R + c.B;
-  const int64_t tiles = (c.capacity + kDecTile - 1) / kDecTile + 1;
-  const int64_t units = row_tiles * c.hkv * tiles;
-  if (units >= (1ll << 31)) return 0;
-  const int64_t most = (units + kDecLeast - 1) / kDecLeast;
-  const int64_t fill = static_cast<int64_t>(st->sm_count) * g_resident[hd == 128][R / 8 - 1];
-  return static_cast<int>(most < fill ? most : fill);
+int launch_kv4_decode(const Kv4AttnArgs& a, int hd, int R, int grid, cudaStream_t s) {
+  if (hd == 128) return R == 8 ? launch_decode<128, 1>(a, grid, s) : launch_decode<128, 2>(a, grid, s);
+  return R == 8 ? launch_decode<64, 1>(a, grid, s) : launch_decode<64, 2>(a, grid, s);
 }
 
 }  // namespace dq
-
-using namespace dq;
-
-static int kv4_rows(int G, int max_new) { return static_cast<int64_t>(G) * max_new <= 8 ? 8 : 16; }
-
-extern "C" size_t dq_kv4_attention_workspace_bytes(const dq_kv4_batch* batch, int hq, int max_new) {
-  DeviceState* st = current_state();
-  Kv4Batch c;
-  if (st == nullptr || kv4_batch_of(batch, &c) != DQ_OK || hq < 1 || max_new < 1) return 0;
-  if (c.B == 0 || c.T == 0) return 0;
-  const int G = hq / c.hkv > 0 ? hq / c.hkv : 1, R = kv4_rows(G, max_new);
-  const int grid = decode_grid(c, G, batch->head_dim, R, st);
-  return kv4_join_bytes(grid) + static_cast<size_t>(grid) * 2 * kv4_partial_floats(R, batch->head_dim) * 4;
-}
-
-extern "C" int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, int64_t q_row_stride, int64_t q_head_stride,
-                                int hq, int max_new, int window, int sinks, float scale, void* out_bf16, void* workspace,
-                                size_t workspace_bytes, void* stream) {
-  DeviceState* st = current_state();
-  if (st == nullptr) return DQ_ERR_NOT_INIT;
-  Kv4AttnArgs a;
-  int rc = kv4_batch_of(batch, &a.c);
-  if (rc != DQ_OK) return rc;
-  if (a.c.B == 0 || a.c.T == 0) return DQ_OK;
-  DQ_REQUIRE(hq >= 1 && hq <= 4096 && hq % a.c.hkv == 0, DQ_ERR_SHAPE, "%d query heads over %d key/value heads", hq, a.c.hkv);
-  DQ_REQUIRE(max_new >= 1 && window >= 0 && sinks >= 0, DQ_ERR_SHAPE, "max_new=%d window=%d sinks=%d", max_new, window, sinks);
-  DQ_REQUIRE(q_bf16 != nullptr && out_bf16 != nullptr, DQ_ERR_NULL, "null pointer");
-  DQ_REQUIRE(static_cast<int64_t>(a.c.T) * hq < (1ll << 30), DQ_ERR_SHAPE, "%d rows of %d heads", a.c.T, hq);
-  DQ_REQUIRE(q_row_stride % 8 == 0 && q_head_stride % 8 == 0 && aligned(q_bf16, 16) && aligned(out_bf16, 16), DQ_ERR_ALIGN,
-             "query heads and outputs must be 16-byte aligned");
-  DQ_REQUIRE(isfinite(scale), DQ_ERR_SHAPE, "scale is not finite");
-  const size_t need = dq_kv4_attention_workspace_bytes(batch, hq, max_new);
-  DQ_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr) && aligned(workspace, 16), DQ_ERR_WORKSPACE,
-             "workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  a.m.window = window < kKv4Far ? window : kKv4Far;
-  a.m.sinks = sinks < kKv4Far ? sinks : kKv4Far;
-  a.q = static_cast<const unsigned short*>(q_bf16);
-  a.q_row = q_row_stride;
-  a.q_head = q_head_stride;
-  a.out = static_cast<unsigned short*>(out_bf16);
-  a.g.G = hq / a.c.hkv;
-  a.g.by = kv4_div(a.g.G);
-  a.scale2 = scale * 1.4426950408889634f;
-  const int R = kv4_rows(a.g.G, max_new), hd = batch->head_dim;
-  const int grid = decode_grid(a.c, a.g.G, hd, R, st);
-  DQ_REQUIRE(grid > 0, DQ_ERR_SHAPE, "%d rows over %d sequences of up to %d tokens are too many for one call", a.c.T, a.c.B,
-             a.c.capacity);
-  a.grid = kv4_div(grid);
-  a.join = static_cast<Kv4Join*>(workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kv4_join_bytes(grid));
-  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (hd == 128) return R == 8 ? launch_decode<128, 1>(a, grid, cs) : launch_decode<128, 2>(a, grid, cs);
-  return R == 8 ? launch_decode<64, 1>(a, grid, cs) : launch_decode<64, 2>(a, grid, cs);
-}

@@ -1,0 +1,557 @@
+// Attention of many query rows per sequence over the paged 4-bit cache (prompts, pieces of prompts) on tcgen05.
+//
+// A segment has up to 256 query rows, (token, query head) pairs of one key/value head: two tiles of 128 rows against the same
+// keys and values, tiles of 128 tokens.  One persistent CTA per SM, sixteen warps:
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: queries into shared memory, scores out of tensor memory, the
+//                    running maximum and sum, weights back to tensor memory, at the end the output
+//   warps 8-11       codes from the pages to fp16 keys and values (fma(c, scale, zero), one rounding) in shared memory
+//   warp 12          issues the products: S = Q K' (both from shared memory), O += P V (P from tensor memory)
+// While the tensor cores work for one row tile, the exponentials of the other are taken: 128 x 128 products of depth 128 take
+// 512 cycles, twice a row tile and token tile, and so do 128 x 128 exponentials at 16 a cycle, so the two pipes would be busy
+// alike.  Tensor memory (512 columns): S0, S1 (the weights take the first half of their scores' columns), O0, O1.
+//
+// Operands are fp16: a key or value of the cache is c * scale + zero with fp16 scale and zero, and 11 bits keep that to 2^-11
+// where bf16 would give 2^-8; queries (bf16) are exact in fp16 times a power of two of their row; weights lie in [0, 2^8].
+// Keys, values and queries hold the elements of each group of eight in the order 0 4 1 5 2 6 3 7, in which nibbles come out of a
+// word two at a time; outputs undo it.  The running maximum m moves only where a row would pass 2^8 above it.
+#include "kv4.cuh"
+
+namespace dq {
+
+constexpr int kPreThreads = 512;
+constexpr int kPreStages = 2;
+
+template <int HD>
+struct PreSmem {
+  static constexpr int kHalf = 128 * 128;              // 128 rows of 64 fp16 elements, 128-byte swizzle
+  static constexpr int kOperand = HD / 64 * kHalf;     // one tile of queries, keys or values
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = 2 * kOperand;
+  static constexpr int kOffV = kOffK + kPreStages * kOperand;
+  static constexpr int kOffBar = kOffV + kPreStages * kOperand;
+  static constexpr int kBars = 2 + 4 * kPreStages + 2 + 2 + 2;
+  static constexpr int kOffValid = kOffBar + kBars * 8;
+  static constexpr int kOffCursor = kOffValid + 4 * 4;
+  static constexpr int kOffTmem = kOffCursor + static_cast<int>((sizeof(Kv4Cursor) + 8 + 15) / 16 * 16);
+  static constexpr int kBytes = kOffTmem + 16 + 1024;  // (the operands start at a multiple of 1024)
+};
+
+// Instruction descriptor, kind::f16: fp16 A and B, fp32 accumulator.  b_rows: B's rows (the sum's index) are contiguous in N.
+__host__ __device__ constexpr uint32_t pre_idesc(int m, int n, bool b_rows) {
+  return (1u << 4) | (b_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// Shared-memory descriptor of values as B of O += P V: rows are tokens (the sum's index), 64 head elements of a row are 128
+// swizzled bytes; eight tokens are 1024 bytes, the next 64 elements kHalf bytes away.
+__device__ __forceinline__ uint64_t pre_desc_rows(uint32_t smem_addr, uint32_t next_block) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(next_block >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+__device__ __forceinline__ void pre_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pre_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pre_tmem_st_x16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ float pre_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pre_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pre_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// eight codes -> fp16 c * scale + zero, elements 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 pre_expand(uint32_t w, __half2 s, __half2 z) {
+  const __half2 k1024 = __half2half2(__ushort_as_half(0x6400)), k16th = __half2half2(__ushort_as_half(0x2C00)),
+                m64 = __half2half2(__ushort_as_half(0xD400));
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t v = w >> (8 * i);
+    const uint32_t lo = (v & 0x000F000Fu) | 0x64006400u, hi = (v & 0x00F000F0u) | 0x64006400u;  // 1024 + c, 1024 + 16 c
+    const __half2 c0 = __hsub2(*reinterpret_cast<const __half2*>(&lo), k1024);                   // exact
+    const __half2 c1 = __hfma2(*reinterpret_cast<const __half2*>(&hi), k16th, m64);              // exact
+    const __half2 x0 = __hfma2(c0, s, z), x1 = __hfma2(c1, s, z);
+    r[2 * i] = *reinterpret_cast<const uint32_t*>(&x0);
+    r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&x1);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPreThreads, 1)
+kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
+  grid_dep_launch_dependents();
+  using L = PreSmem<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ volatile int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* q_full = bar;                       // [2] a row tile's queries are in shared memory
+  uint64_t* k_full = bar + 2;                   // [stage]
+  uint64_t* k_empty = k_full + kPreStages;
+  uint64_t* v_full = k_empty + kPreStages;
+  uint64_t* v_empty = v_full + kPreStages;
+  uint64_t* s_full = v_empty + kPreStages;      // [2] scores of a row tile are in tensor memory
+  uint64_t* p_full = s_full + 2;                // [2] its weights are
+  uint64_t* o_done = p_full + 2;                // [2] a tile's values are in its output
+  // pieces of 16 tokens that are there, of the last four tiles: two bits in each of four bytes (warps 8 to 11)
+  volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kOffValid);
+  Kv4Cursor& found = *reinterpret_cast<Kv4Cursor*>(smem + L::kOffCursor);
+  int* s_share = reinterpret_cast<int*>(&found + 1);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 128);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_done + i, 1);
+    }
+    for (int i = 0; i < kPreStages; ++i) {
+      mbar_init(k_full + i, 128);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 128);
+      mbar_init(v_empty + i, 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(s_tmem, 512);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  if (warp == 0) {
+    const Kv4Start k = kv4_begin_any<kPreTile>(a.c, a.m, a.g, kPreRows, kPreLeast, a.grid, lane);
+    if (lane == 0) {
+      if (k.any) found = k.k;
+      else a.join[blockIdx.x].parts = 0;
+      *s_share = k.any ? k.share : 0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const int share = *s_share;
+  const uint32_t base = smem_u32(smem);
+  if (share == 0) {
+    if (warp == 12) tmem_dealloc(tmem, 512);
+    return;
+  }
+  Kv4Cursor at = found;
+  bool ok = true;  // no wait has run out
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------------------------------------ softmax
+    const int tile = warp >> 2, row_in = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes, in the upper half of an address
+    const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
+    uint32_t s_phase = 0;  // token tiles so far
+    int seen = 0;          // token tiles of the call, both row tiles'
+    bool is_first = true, goes_on = false;
+    for (;; is_first = false) {
+      const int rows = at.seq.n * a.g.G - at.rt * kPreRows;  // of the segment, 256 at most count
+      const int n_tiles = at.u1 - at.u0;
+      const int r = at.rt * kPreRows + tile * 128 + row_in;
+      const bool there = tile * 128 + row_in < rows;
+      const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
+      const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
+      if (tile == 0 || rows > 128) {
+        float mul = 1.0f;
+        bool finite = true;
+        {
+          // the row as fp16 times a power of two that brings its largest element to [2^14, 2^15)
+          const unsigned short* src = a.q + static_cast<int64_t>(at.seq.row0 + i_tok) * a.q_row + static_cast<int64_t>(head) * a.q_head;
+          uint4 v[HD / 8];
+          uint32_t big = 0;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (there) v[i] = *reinterpret_cast<const uint4*>(src + 8 * i);
+          }
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i)
+            big = __vmaxu2(__vmaxu2(__vmaxu2(big, v[i].x & 0x7FFF7FFFu), __vmaxu2(v[i].y & 0x7FFF7FFFu, v[i].z & 0x7FFF7FFFu)),
+                           v[i].w & 0x7FFF7FFFu);
+          big = max(big & 0xFFFFu, big >> 16);
+          finite = big < 0x7F80u;
+          const int e = big > 0 && finite ? static_cast<int>(big >> 7) - 127 : 0;
+          const int up = max(min(14 - e, 100), -103);
+          float by = __int_as_float((up + 127) << 23);
+          mul = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
+          if (a.scale2 < 0.0f) by = -by;                    // (the maximum is taken of scores times |scale|)
+          if (a.scale2 == 0.0f || !finite) by = 0.0f, mul = 1.0f;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              // elements 2j, 2j + 1 and 2j + 4, 2j + 5; (x * 0 is NaN for an element that is not finite: such rows are made zero)
+              const uint32_t p = finite ? w[j] : 0u, q = finite ? w[j + 2] : 0u;
+              h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
+              h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
+            }
+            *reinterpret_cast<uint4*>(smem + L::kOffQ + tile * L::kOperand + (i >> 3) * L::kHalf + row_in * 128 +
+                                      (((i & 7) ^ (row_in & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(q_full + tile);
+        }
+        const int kv = min(at.seq.kv, a.c.capacity);
+        const int p_row = at.seq.kv - at.seq.n + i_tok;
+        const int hi = there ? min(p_row + 1, kv) : 0;                   // tokens lo ... hi - 1 and those below `first`
+        const int lo = a.m.window > 0 ? p_row - a.m.window + 1 : 0;
+        const int first = a.m.window > 0 ? min(a.m.sinks, hi) : 0;
+        float m = kKv4NoMax;
+        float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          const int tok = at.span.tile(at.u0 + j) * kPreTile;
+          ok = mbar_wait(s_full + tile, s_phase & 1, &s_abort, 42);
+          tc_fence_after();
+          const uint32_t got = valid[(seen + j) & 3];
+          const bool whole = got == 0x03030303u && tok + kPreTile <= kv && tok + kPreTile <= at.span.p_lo + 1 &&
+                             (a.m.window == 0 || tok > at.span.p_hi - a.m.window || tok + kPreTile <= a.m.sinks);
+          // Scores are read twice, 32 at a time, for the maximum and for the weights: 128 of them in registers would leave the
+          // converting warps too few.
+          auto hide = [&](uint32_t (&s)[32], int c0) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const int t = tok + c0 + c;
+              const bool see = t < hi && (t >= lo || t < first) && ((got >> ((c0 >> 5) * 8 + (c >> 4))) & 1u);
+              if (!see) s[c] = 0xFF800000u;
+            }
+          };
+          uint32_t s[2][32];
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_ld_x32(t_s, s[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            if (c < 3) tmem_ld_x32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
+            if (!whole) hide(s[c & 1], 32 * c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+              for (int f = 0; f < 4; ++f)
+                top[f] = fmaxf(top[f], fmaxf(__uint_as_float(s[c & 1][e + f]), __uint_as_float(s[c & 1][e + f + 4])));
+          }
+          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
+          tmem_ld_x32(t_s, s[0]);
+          if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
+            const float to = fmaxf(m, high), by = pre_exp2(m - to);
+            m = to;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) l2[e].x *= by, l2[e].y *= by;
+            if (j > 0) {
+              ok = ok && mbar_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the tile before is in O
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < HD; c += 16) {
+                uint32_t o[16];
+                tmem_ld_x16(t_o + c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+                pre_tmem_st_x16(t_o + c, o);
+              }
+            }
+          }
+          const float2 mul2 = make_float2(mul, mul), low = make_float2(-m, -m);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            if (c < 3) tmem_ld_x32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
+            if (!whole) hide(s[c & 1], 32 * c);
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 x =
+                  __ffma2_rn(make_float2(__uint_as_float(s[c & 1][2 * e]), __uint_as_float(s[c & 1][2 * e + 1])), mul2, low);
+              const float2 w = make_float2(pre_exp2(x.x), pre_exp2(x.y));
+              l2[e & 1] = __fadd2_rn(l2[e & 1], w);
+              p[e] = pre_half2(w.x, w.y);
+            }
+            pre_tmem_st_x16(t_s + 16 * c, p);  // (columns whose scores have been read)
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(p_full + tile);
+          ++s_phase;
+        }
+        // output of the row
+        const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+        ok = ok && mbar_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 44);
+        tc_fence_after();
+        const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
+        // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
+        float by = whole_segment ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
+        if (!finite && l != 0.0f) by = __int_as_float(0x7FC00000);
+        float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(kPreRows, HD);
+        float* part_o = part + 2 * kPreRows + (tile * 128 + row_in) * HD;
+#pragma unroll
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld_x32(t_o + c, o);
+          tmem_ld_wait();
+          if (there && ok) {
+#pragma unroll
+            for (int g = 0; g < 32; g += 8) {
+              float v[8];  // elements in their own order
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] = __uint_as_float(o[g + 2 * e]) * by;
+                v[e + 4] = __uint_as_float(o[g + 2 * e + 1]) * by;
+              }
+              if (l == 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+              }
+              if (whole_segment) {
+                *reinterpret_cast<uint4*>(a.out + out_at + c + g) =
+                    make_uint4(pre_bf16x2(v[0], v[1]), pre_bf16x2(v[2], v[3]), pre_bf16x2(v[4], v[5]), pre_bf16x2(v[6], v[7]));
+              } else {
+                *reinterpret_cast<float4*>(part_o + c + g) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(part_o + c + g + 4) = make_float4(v[4], v[5], v[6], v[7]);
+              }
+            }
+          }
+        }
+        if (!whole_segment && there) {
+          part[2 * (tile * 128 + row_in)] = m;
+          part[2 * (tile * 128 + row_in) + 1] = l;
+        }
+        tc_fence_before();  // (the next segment's products over O come behind this row's next arrival)
+      }
+      seen += n_tiles;
+      const bool begins = at.u0 == 0 && at.u1 < at.span.count;
+      if (begins && threadIdx.x == 0) {
+        Kv4Join j;
+        j.parts = 1 + (at.span.count - at.u1 + share - 1) / share;
+        j.slot = is_first ? 0 : 1;
+        j.rows = min(rows, kPreRows);
+        j.first_row = at.rt * kPreRows;
+        j.row0 = at.seq.row0;
+        j.h = at.h;
+        a.join[blockIdx.x] = j;
+      }
+      goes_on |= begins;
+      if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
+    }
+    if (threadIdx.x == 0 && !goes_on) a.join[blockIdx.x].parts = 0;
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------------------------------------ keys and values
+    constexpr int kLanes = HD / 32;           // lanes with 16 bytes of codes each to a token
+    constexpr int kStep = 32 / kLanes;        // tokens of a warp per load
+    constexpr int kLoads = 32 / kStep;        // loads for the warp's 32 tokens
+    const int w = warp - 8, q = lane % kLanes, in = lane / kLanes;
+    const int P = 1 << a.c.page_shift;
+    struct Raw {
+      uint4 code[kLoads];
+      __half2 pair[kLoads];
+    } rk, rv;
+    bool more = true;
+    int u = at.u0;
+    uint32_t got = 0;               // this warp's two pieces of 16 tokens
+    const uint8_t* block[2];        // of the tile that is loaded next
+    int slot[2], left = 0;          // left: tokens of the tile from this warp's first one on
+    auto seek = [&]() {
+      while (more && u >= at.u1) {
+        more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at);
+        u = at.u0;
+      }
+      got = 0;
+      if (!more) return;
+      const int tok = at.span.tile(u) * kPreTile + w * 32;
+      left = min(at.seq.kv, a.c.capacity) - tok;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = tok + 16 * i;
+        int page = -1;
+        if (16 * i < left) page = a.c.table[at.b * a.c.table_stride + (t >> a.c.page_shift)];
+        if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.c.num_pages)) got |= 1u << i;
+        block[i] = a.c.pages + static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.c.page_stride) +
+                   static_cast<int64_t>(at.h) * P * (HD + 8);
+        slot[i] = t & (P - 1);
+      }
+      ++u;
+    };
+    // tokens that are not there become zeros (their weights are zero, and zero times anything that a page may hold is not)
+    auto load = [&](Raw& r, bool values) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int t = i * kStep + in, piece = (i * kStep) >> 4;  // (16 tokens are a multiple of kStep)
+        r.code[i] = make_uint4(0, 0, 0, 0);
+        r.pair[i] = __half2half2(__ushort_as_half(0));
+        if (((got >> piece) & 1u) && t < left) {
+          const int sl = slot[piece] + (t & 15);
+          r.code[i] = *reinterpret_cast<const uint4*>(block[piece] + (values ? P * (HD / 2) : 0) + sl * (HD / 2) + q * 16);
+          r.pair[i] = *reinterpret_cast<const __half2*>(block[piece] + P * HD + (values ? 4 * P : 0) + sl * 4);
+        }
+      }
+    };
+    auto store = [&](const Raw& r, uint8_t* dst) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int t = w * 32 + i * kStep + in;
+        const __half2 s = __low2half2(r.pair[i]), z = __high2half2(r.pair[i]);
+        uint32_t c[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
+        // lanes of the second 64 elements take their words in the order 2 3 0 1: the eight lanes that store together
+        // hit eight different 16-byte columns
+        const int turn = q & 2;
+        if (turn) {
+          uint32_t x = c[0];
+          c[0] = c[2], c[2] = x;
+          x = c[1];
+          c[1] = c[3], c[3] = x;
+        }
+        uint8_t* row = dst + (q >> 1) * L::kHalf + t * 128;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(row + (((((q & 1) << 2) + (e ^ turn)) ^ (t & 7)) << 4)) = pre_expand(c[e], s, z);
+      }
+      fence_proxy_async_smem();
+    };
+    seek();
+    load(rk, false);
+    load(rv, true);
+    for (uint32_t n = 0; more && ok; ++n) {
+      const int stage = n % kPreStages;
+      const uint32_t parity = ((n / kPreStages) & 1) ^ 1;
+      const uint32_t mine = got;
+      ok = mbar_wait(k_empty + stage, parity, &s_abort, 45);
+      // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
+      if (lane == 0) reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(mine);
+      store(rk, smem + L::kOffK + stage * L::kOperand);
+      mbar_arrive(k_full + stage);
+      const Raw now = rv;
+      seek();
+      if (more) load(rk, false);
+      ok = ok && mbar_wait(v_empty + stage, parity, &s_abort, 46);
+      store(now, smem + L::kOffV + stage * L::kOperand);
+      mbar_arrive(v_full + stage);
+      if (more) load(rv, true);
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------------------------------------------ products
+    if (elect_one()) {
+      constexpr uint32_t kIdescS = pre_idesc(128, 128, false), kIdescO = pre_idesc(128, HD, true);
+      uint32_t q_phase = 0, q1_phase = 0, p_phase0 = 0, p_phase1 = 0, n = 0;  // n: token tiles so far
+      auto scores = [&](int tile, uint32_t stage) {
+        const uint32_t qa = base + L::kOffQ + tile * L::kOperand, ka = base + L::kOffK + stage * L::kOperand;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          pre_mma_ss(tmem + tile * 128, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
+                     umma_desc_k_sw128(ka + (k >> 2) * L::kHalf + (k & 3) * 32), kIdescS, k > 0);
+        umma_commit(s_full + tile);
+      };
+      auto values = [&](int tile, uint32_t stage, bool add) {
+        const uint32_t va = base + L::kOffV + stage * L::kOperand;
+#pragma unroll
+        for (int k = 0; k < kPreTile / 16; ++k)
+          pre_mma_ts(tmem + 256 + tile * HD, tmem + tile * 128 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf), kIdescO,
+                     add || k > 0);
+        umma_commit(o_done + tile);
+      };
+      for (;;) {
+        const int rows = at.seq.n * a.g.G - at.rt * kPreRows, n_tiles = at.u1 - at.u0;
+        const bool two = rows > 128;
+        ok = ok && mbar_wait(q_full, q_phase & 1, &s_abort, 47);
+        ++q_phase;
+        if (two) {
+          ok = ok && mbar_wait(q_full + 1, q1_phase & 1, &s_abort, 48);
+          ++q1_phase;
+        }
+        ok = ok && mbar_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
+        if (!ok) break;
+        tc_fence_after();
+        scores(0, n % kPreStages);
+        if (two) scores(1, n % kPreStages);
+        umma_commit(k_empty + n % kPreStages);
+        for (int j = 0; j < n_tiles && ok; ++j, ++n) {
+          const uint32_t stage = n % kPreStages, next = (n + 1) % kPreStages;
+          const bool last = j + 1 == n_tiles;
+          ok = mbar_wait(v_full + stage, (n / kPreStages) & 1, &s_abort, 50);
+          ok = ok && mbar_wait(p_full, p_phase0 & 1, &s_abort, 51);
+          ++p_phase0;
+          tc_fence_after();
+          if (!ok) break;
+          values(0, stage, j > 0);
+          if (!last) {
+            ok = mbar_wait(k_full + next, ((n + 1) / kPreStages) & 1, &s_abort, 52);
+            if (!ok) break;
+            tc_fence_after();
+            scores(0, next);
+          }
+          if (two) {
+            ok = mbar_wait(p_full + 1, p_phase1 & 1, &s_abort, 53);
+            ++p_phase1;
+            if (!ok) break;
+            tc_fence_after();
+            values(1, stage, j > 0);
+          }
+          umma_commit(v_empty + stage);
+          if (!last) {
+            if (two) scores(1, next);
+            umma_commit(k_empty + next);
+          }
+        }
+        if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
+      }
+    }
+    __syncwarp();
+  }
+  // every product has been waited for by the softmax of its row tile (or a wait ran out)
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && s_abort != 0) atomicExch(status, s_abort);
+}
+
+template <int HD>
+static int init_prefill() {
+  DQ_CHECK_CUDA(cudaFuncSetAttribute(kv4_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, PreSmem<HD>::kBytes));
+  return DQ_OK;
+}
+int init_kv4_prefill_kernels() {
+  const int rc = init_prefill<64>();
+  return rc == DQ_OK ? init_prefill<128>() : rc;
+}
+int launch_kv4_prefill(const Kv4AttnArgs& a, int hd, int grid, cudaStream_t s, DeviceState* st) {
+  if (hd == 128)
+    DQ_CHECK_CUDA(launch_pdl(kv4_prefill_kernel<128>, dim3(grid), dim3(kPreThreads), PreSmem<128>::kBytes, s, a, st->status_dev));
+  else
+    DQ_CHECK_CUDA(launch_pdl(kv4_prefill_kernel<64>, dim3(grid), dim3(kPreThreads), PreSmem<64>::kBytes, s, a, st->status_dev));
+  return DQ_OK;
+}
+
+}  // namespace dq

@@ -50,19 +50,20 @@ def attention(q, ks, vs, new, lengths, window=0, sinks=0, scale=None, missing=No
     first = 0
     for b, (n, m) in enumerate(zip(new, lengths)):
         k, v = ks[b], vs[b]
-        L, hkv = k.shape[1], k.shape[0]
-        for i in range(n):
-            p = m - n + i
-            see = [j for j in range(max(0, min(p + 1, L))) if window == 0 or j > p - window or j < sinks]
-            if missing is not None:
-                see = [j for j in see if not missing(b, j)]
-            if not see:
-                continue
-            at = torch.tensor(see, device=q.device)
-            kk, vv = k[:, at], v[:, at]
-            x = q[first + i].double().view(hkv, hq // hkv, hd)
-            w = torch.softmax(torch.einsum("hgd,hjd->hgj", x, kk) * scale, dim=-1)
-            out[first + i] = torch.einsum("hgj,hjd->hgd", w, vv).reshape(hq, hd)
+        hkv, L = k.shape[0], min(k.shape[1], max(m, 0))
+        if n and L:
+            j = torch.arange(L, device=q.device)
+            gone = torch.tensor([missing is not None and missing(b, t) for t in range(L)], device=q.device)
+            for at in range(0, n, 256):
+                p = (m - n + torch.arange(at, min(n, at + 256), device=q.device))[:, None]
+                see = (j <= p) & ~gone
+                if window:
+                    see &= (j > p - window) | (j < sinks)
+                x = q[first + at : first + at + len(p)].double().view(len(p), hkv, hq // hkv, hd)
+                w = torch.einsum("ihgd,hjd->hgij", x, k[:, :L]) * scale
+                w = torch.softmax(w.masked_fill(~see, -math.inf), dim=-1)
+                w = torch.where(see.any(-1)[:, None], w, torch.zeros_like(w))
+                out[first + at : first + at + len(p)] = torch.einsum("hgij,hjd->ihgd", w, v[:, :L]).reshape(len(p), hq, hd)
         first += n
     return out
 

@@ -148,13 +148,15 @@ def test_append_skips_tokens_without_a_place_and_leaves_rows_behind_the_last_seq
 
 # ------------------------------------------------------------------------------------------------ attention
 def run_attention(hq, hkv, hd, page, new, lengths, window=0, sinks=0, seed=5, q_scale=1.5, scale=None, spread=1.0,
-                  zero_scale=False, max_new=None, uniform=False):
+                  zero_scale=False, max_new=None, uniform=False, keys_fp16=False):
     gen = torch.Generator().manual_seed(seed)
     pages, table, ks, vs = ref.make_cache(gen, len(new), lengths, hkv, hd, page, spread=spread, zero_scale=zero_scale)
     q = (torch.randn(sum(new), hq, hd, generator=gen) * q_scale).to(torch.bfloat16).cuda()
     cache = ops.KV4Cache(pages, hd, page)
     got = ops.kv4_attention(q, cache, table, i32(lengths), cu_new=None if uniform else cu_of(new),
                             max_new=max_new if max_new is not None else max(new), window=window, sinks=sinks, scale=scale)
+    if keys_fp16:
+        ks = [k.half().double() for k in ks]
     want = ref.attention(q, ks, vs, new, lengths, window, sinks, scale)
     tol = ref.attention_tolerance(want, vs, lengths)
     err = (got.double() - want).abs()
@@ -184,6 +186,33 @@ def test_attention_of_a_few_rows(hq, hkv, hd, page, new, lengths):
     run_attention(hq, hkv, hd, page, new, lengths)
 
 
+PROMPTS = [
+    # hq, hkv, hd, page, new, lengths
+    (4, 1, 128, 16, [5], [5]),
+    (4, 1, 64, 16, [32], [32]),                        # one full row tile
+    (4, 1, 128, 64, [33], [33]),                       # one row more
+    (8, 2, 128, 32, [64, 64], [64, 127]),              # both row tiles of a segment full
+    (8, 2, 64, 16, [65, 1, 0, 130], [128, 1, 0, 131]),
+    (28, 4, 128, 64, [100, 37, 256], [100, 700, 300]),  # seven heads in a group
+    (3, 3, 128, 256, [129, 257, 300], [129, 1000, 301]),
+    (16, 1, 64, 128, [200], [1333]),
+    (8, 2, 128, 16, [1] * 9 + [90], [1 + 50 * i for i in range(9)] + [450]),  # a prompt among single tokens
+    (32, 8, 128, 64, [700, 900], [700, 1500]),
+    (2, 2, 64, 32, [50] * 140, [50 + i for i in range(140)]),
+]
+
+
+@pytest.mark.parametrize("hq,hkv,hd,page,new,lengths", PROMPTS)
+def test_attention_of_many_rows(hq, hkv, hd, page, new, lengths):
+    run_attention(hq, hkv, hd, page, new, lengths)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 4), (40, 1), (128, 0), (129, 130), (300, 64), (5000, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
+@pytest.mark.parametrize("hd,page", [(128, 16), (64, 128)])
+def test_attention_of_many_rows_with_a_window_and_sinks(hd, page, window, sinks):
+    run_attention(8, 2, hd, page, [90, 1, 300, 33], [90, 70, 713, 900], window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 4), (7, 1), (64, 0), (64, 33), (200, 64), (5000, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
 @pytest.mark.parametrize("hd,page", [(128, 16), (64, 128)])
 def test_attention_with_a_window_and_sinks(hd, page, window, sinks):
@@ -191,44 +220,59 @@ def test_attention_with_a_window_and_sinks(hd, page, window, sinks):
 
 
 @pytest.mark.parametrize("spread", [1e-5, 1e-3, 30.0, 1000.0])
-def test_attention_over_values_of_other_sizes(spread):
-    run_attention(8, 2, 128, 32, [1, 1], [400, 77], spread=spread, q_scale=0.5 / spread if spread > 1 else 1.0)
+@pytest.mark.parametrize("new", [[1, 1], [50, 9]])
+def test_attention_over_values_of_other_sizes(spread, new):
+    run_attention(8, 2, 128, 32, new, [400, 77], spread=spread, q_scale=0.5 / spread if spread > 1 else 1.0)
 
 
-def test_attention_over_constant_heads():
-    run_attention(8, 2, 128, 32, [1, 1], [400, 77], zero_scale=True)
+@pytest.mark.parametrize("new", [[1, 1], [50, 9]])
+def test_attention_over_constant_heads(new):
+    run_attention(8, 2, 128, 32, new, [400, 77], zero_scale=True)
 
 
 @pytest.mark.parametrize("q_scale", [1e-20, 1e-4, 20.0])
-def test_attention_of_small_and_large_queries(q_scale):
-    run_attention(8, 2, 128, 32, [1, 2], [200, 77], q_scale=q_scale)
+@pytest.mark.parametrize("new", [[1, 2], [70, 9]])
+def test_attention_of_small_and_large_queries(q_scale, new):
+    # Many rows take keys as fp16(c * scale + zero), 2^-11 of an element.  With q of size 20 and k of size 2 a score of 128 terms
+    # moves by 20 * 2 * 2^-12 * sqrt(128) / sqrt(128) = 0.01, a weight by 1 %, above the tolerance: the reference takes them so too.
+    run_attention(8, 2, 128, 32, new, [200, 77], q_scale=q_scale, keys_fp16=max(new) * 4 > 16)
 
 
-def test_attention_takes_a_scale():
-    run_attention(8, 2, 128, 32, [1, 2], [200, 77], scale=0.31)
-    run_attention(8, 2, 64, 32, [1, 2], [200, 77], scale=-0.1)
-    run_attention(8, 2, 64, 32, [1, 2], [200, 77], scale=0.0)
+@pytest.mark.parametrize("new", [[1, 2], [70, 9]])
+def test_attention_takes_a_scale(new):
+    run_attention(8, 2, 128, 32, new, [200, 77], scale=0.31, keys_fp16=max(new) * 4 > 16)  # (as above: scores of size 10)
+    run_attention(8, 2, 64, 32, new, [200, 77], scale=-0.1)
+    run_attention(8, 2, 64, 32, new, [200, 77], scale=0.0)
 
 
-def test_attention_one_long_sequence_over_every_cta():
-    run_attention(8, 2, 128, 32, [1], [40001])
+@pytest.mark.parametrize("new", [[1], [3], [20], [80]])
+def test_attention_one_long_sequence_over_every_cta(new):
+    run_attention(8, 2, 128, 32, new, [40001])
 
 
 def test_attention_without_row_offsets():
     run_attention(8, 2, 128, 32, [2] * 7, [200, 77, 2, 1000, 64, 65, 66], uniform=True)
+    run_attention(8, 2, 128, 32, [40] * 7, [200, 77, 40, 1000, 64, 65, 66], uniform=True)
 
 
-def test_attention_gives_the_same_bits_again():
+@pytest.mark.parametrize("most", [1, 3, 1000])
+def test_more_or_fewer_rows_than_the_hint(most):
+    run_attention(8, 2, 128, 32, [9, 1, 30], [200, 77, 64], max_new=most)
+
+
+@pytest.mark.parametrize("each", [1, 60])
+def test_attention_gives_the_same_bits_again(each):
     gen = torch.Generator().manual_seed(6)
     pages, table, ks, vs = ref.make_cache(gen, 3, [5000, 100, 9000], 2, 128, 32)
-    q = torch.randn(3, 8, 128, generator=gen).to(torch.bfloat16).cuda()
+    q = torch.randn(3 * each, 8, 128, generator=gen).to(torch.bfloat16).cuda()
     cache, n = ops.KV4Cache(pages, 128, 32), i32([5000, 100, 9000])
     first = ops.kv4_attention(q, cache, table, n)
     for _ in range(5):
         assert torch.equal(first, ops.kv4_attention(q, cache, table, n))
 
 
-def test_attention_rows_that_see_nothing_are_zero_and_pages_that_are_not_there_are_not_seen():
+@pytest.mark.parametrize("most", [4, 100])
+def test_attention_rows_that_see_nothing_are_zero_and_pages_that_are_not_there_are_not_seen(most):
     gen = torch.Generator().manual_seed(7)
     hq, hkv, hd, page = 8, 2, 128, 16
     lengths, new = [0, 2, 200, 40], [1, 4, 2, 1]  # no token; two rows before the first token
@@ -236,30 +280,32 @@ def test_attention_rows_that_see_nothing_are_zero_and_pages_that_are_not_there_a
     table[2, 3], table[2, 4] = -7, pages.shape[0]  # tokens 48 ... 79 of sequence 2
     table[3] = -1
     q = torch.randn(sum(new), hq, hd, generator=gen).to(torch.bfloat16).cuda()
-    got = ops.kv4_attention(q, ops.KV4Cache(pages, hd, page), table, i32(lengths), cu_new=cu_of(new), max_new=4)
+    got = ops.kv4_attention(q, ops.KV4Cache(pages, hd, page), table, i32(lengths), cu_new=cu_of(new), max_new=most)
     want = ref.attention(q, ks, vs, new, lengths, missing=lambda b, j: b == 3 or (b == 2 and 48 <= j < 80))
     assert bool((want[[0, 1, 2, 7]] == 0).all()) and bool((got[[0, 1, 2, 7]] == 0).all())
     assert bool(((got.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths)).all())
 
 
-def test_attention_reads_nothing_behind_the_table_row():
+@pytest.mark.parametrize("most", [None, 100])
+def test_attention_reads_nothing_behind_the_table_row(most):
     gen = torch.Generator().manual_seed(8)
     pages, table, ks, vs = ref.make_cache(gen, 2, [64, 64], 2, 128, 16)
     q = torch.randn(2, 4, 128, generator=gen).to(torch.bfloat16).cuda()
     cache = ops.KV4Cache(pages, 128, 16)
     # two pages of each sequence's row, and a length that passes them: tokens 32 ... are not there
-    got = ops.kv4_attention(q, cache, table[:, :2], i32([64, 2 ** 31 - 1]))
+    got = ops.kv4_attention(q, cache, table[:, :2], i32([64, 2 ** 31 - 1]), max_new=most)
     want = ref.attention(q, [k[:, :32] for k in ks], [v[:, :32] for v in vs], [1, 1], [64, 10 ** 9])
     want[1] = ref.attention(q[1:], [ks[1][:, :32]], [vs[1][:, :32]], [1], [64])[0]
     assert bool(((got.double() - want).abs() <= ref.attention_tolerance(want, vs, [64])).all())
 
 
-def test_attention_keeps_a_row_that_is_not_finite_to_itself():
+@pytest.mark.parametrize("most", [None, 100])
+def test_attention_keeps_a_row_that_is_not_finite_to_itself(most):
     gen = torch.Generator().manual_seed(9)
     pages, table, ks, vs = ref.make_cache(gen, 2, [100, 100], 1, 64, 16)
     q = torch.randn(2, 4, 64, generator=gen).to(torch.bfloat16).cuda()
     q[0, 1, 3], q[0, 2, 5] = float("nan"), float("inf")
-    got = ops.kv4_attention(q, ops.KV4Cache(pages, 64, 16), table, i32([100, 100]))
+    got = ops.kv4_attention(q, ops.KV4Cache(pages, 64, 16), table, i32([100, 100]), max_new=most)
     assert bool(got[0, 1:3].isnan().all())
     q[0, 1:3] = 0
     want = ref.attention(q, ks, vs, [1, 1], [100, 100])
@@ -268,12 +314,13 @@ def test_attention_keeps_a_row_that_is_not_finite_to_itself():
     assert all(bool(((got[i].double() - want[i]).abs() <= tol[i]).all()) for i in keep)
 
 
-def test_attention_leaves_rows_behind_the_last_sequence():
+@pytest.mark.parametrize("most", [3, 100])
+def test_attention_leaves_rows_behind_the_last_sequence(most):
     gen = torch.Generator().manual_seed(10)
     pages, table, ks, vs = ref.make_cache(gen, 2, [100, 50], 2, 64, 16)
     q = torch.randn(9, 4, 64, generator=gen).to(torch.bfloat16).cuda()
     out = torch.full((9, 4, 64), 3.0, dtype=torch.bfloat16, device="cuda")
-    back = ops.kv4_attention(q, ops.KV4Cache(pages, 64, 16), table, i32([100, 50]), cu_new=i32([0, 2, 5]), max_new=3, out=out)
+    back = ops.kv4_attention(q, ops.KV4Cache(pages, 64, 16), table, i32([100, 50]), cu_new=i32([0, 2, 5]), max_new=most, out=out)
     assert back.data_ptr() == out.data_ptr() and bool((out[5:] == 3.0).all())
     want = ref.attention(q[:5], ks, vs, [2, 3], [100, 50])
     assert bool(((out[:5].double() - want).abs() <= ref.attention_tolerance(want, vs, [100])).all())
@@ -295,8 +342,9 @@ def test_attention_takes_strided_queries_layers_of_a_larger_cache_and_sliced_tab
               torch.empty(2, hq, hd + 8, dtype=torch.bfloat16, device="cuda")[..., :hd].copy_(want_q),
               torch.empty(2, hq, hd + 3, dtype=torch.bfloat16, device="cuda")[..., 1 : hd + 1].copy_(want_q),  # not 16-byte
               torch.empty(2, hq, 2 * hd, dtype=torch.bfloat16, device="cuda")[..., ::2].copy_(want_q)):
-        got = ops.kv4_attention(q, cache, wide[:, 2 : 2 + table.shape[1]], i32(lengths))
-        assert bool(((got.double() - want).abs() <= tol).all())
+        for most in (1, 100):
+            got = ops.kv4_attention(q, cache, wide[:, 2 : 2 + table.shape[1]], i32(lengths), max_new=most)
+            assert bool(((got.double() - want).abs() <= tol).all())
 
 
 def test_append_takes_strided_rows():
@@ -406,7 +454,8 @@ def test_a_generation_through_the_cache_matches_attention_over_unquantised_heads
             assert bool(((rows.double() - all_rows).abs() <= 2.0 ** -8 * all_rows.abs() + 1e-5).all())
 
 
-def test_captured_calls_follow_the_lengths_on_the_device_and_graphs_do_not_share():
+@pytest.mark.parametrize("most", [1, 100])
+def test_captured_calls_follow_the_lengths_on_the_device_and_graphs_do_not_share(most):
     gen = torch.Generator().manual_seed(14)
     hq, hkv, hd, page = 8, 2, 128, 16
     lengths = [700, 90]
@@ -414,13 +463,13 @@ def test_captured_calls_follow_the_lengths_on_the_device_and_graphs_do_not_share
     cache, n = ops.KV4Cache(pages, hd, page), i32(lengths)
     q = torch.randn(2, hq, hd, generator=gen).to(torch.bfloat16).cuda()
     qs = [q.clone(), q.clone()]
-    ops.kv4_attention(q, cache, table, n)
+    ops.kv4_attention(q, cache, table, n, max_new=most)
     torch.cuda.synchronize()
     graphs, outs = [], []
     for x in qs:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            outs.append(ops.kv4_attention(x, cache, table, n))
+            outs.append(ops.kv4_attention(x, cache, table, n, max_new=most))
         graphs.append(g)
     for now in ([700, 90], [33, 1], [512, 64]):
         n.copy_(i32(now))
