@@ -2,10 +2,11 @@
 //
 // A segment has up to 256 query rows, (token, query head) pairs of one key/value head: two tiles of 128 rows against the same
 // keys and values, tiles of 128 tokens.  One persistent CTA per SM, sixteen warps:
-//   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: queries into shared memory, scores out of tensor memory, the
-//                    running maximum and sum, weights back to tensor memory, at the end the output
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: scores out of tensor memory, the running maximum and sum,
+//                    weights back to tensor memory, at the end the output
 //   warps 8-11       codes from the pages to fp16 keys and values (fma(c, scale, zero), one rounding) in shared memory
 //   warp 12          issues the products: S = Q K' (both from shared memory), O += P V (P from tensor memory)
+//   warps 13-15      queries of the next segment into shared memory as soon as its predecessor's last scores are computed
 // While the tensor cores work for one row tile, the exponentials of the other are taken: 128 x 128 products of depth 128 take
 // 512 cycles, twice a row tile and token tile, and so do 128 x 128 exponentials at 16 a cycle, so the two pipes would be busy
 // alike.  Tensor memory (512 columns): S0, S1 (the weights take the first half of their scores' columns), O0, O1.
@@ -20,6 +21,7 @@ namespace dq {
 
 constexpr int kPreThreads = 512;
 constexpr int kPreStages = 2;
+constexpr int kPreLoaders = 3;    // warps that bring the queries
 
 template <int HD>
 struct PreSmem {
@@ -28,10 +30,13 @@ struct PreSmem {
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = 2 * kOperand;
   static constexpr int kOffV = kOffK + kPreStages * kOperand;
-  static constexpr int kOffBar = kOffV + kPreStages * kOperand;
-  static constexpr int kBars = 2 + 4 * kPreStages + 2 + 2 + 2;
+  static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
+  static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
+  static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
+  static constexpr int kBars = 4 + 4 * kPreStages + 6 + 8;
   static constexpr int kOffValid = kOffBar + kBars * 8;
-  static constexpr int kOffCursor = kOffValid + 4 * 4;
+  static constexpr int kOffMul = kOffValid + 4 * 4;            // [2][256] what a row's scores have to be multiplied with
+  static constexpr int kOffCursor = kOffMul + 2 * kPreRows * 4;
   static constexpr int kOffTmem = kOffCursor + static_cast<int>((sizeof(Kv4Cursor) + 8 + 15) / 16 * 16);
   static constexpr int kBytes = kOffTmem + 16 + 1024;  // (the operands start at a multiple of 1024)
 };
@@ -71,6 +76,14 @@ __device__ __forceinline__ void pre_tmem_st_x16(uint32_t taddr, const uint32_t* 
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+__device__ __forceinline__ void pre_cp_async_16(uint32_t dst, const void* src, int bytes = 16) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ float pre_exp2(float x) {
   float r;
@@ -115,13 +128,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint64_t* q_full = bar;                       // [2] a row tile's queries are in shared memory
-  uint64_t* k_full = bar + 2;                   // [stage]
+  uint64_t* q_empty = bar + 2;                  // [2] its last scores have been computed
+  uint64_t* k_full = bar + 4;                   // [stage]
   uint64_t* k_empty = k_full + kPreStages;
   uint64_t* v_full = k_empty + kPreStages;
   uint64_t* v_empty = v_full + kPreStages;
   uint64_t* s_full = v_empty + kPreStages;      // [2] scores of a row tile are in tensor memory
   uint64_t* p_full = s_full + 2;                // [2] its weights are
   uint64_t* o_done = p_full + 2;                // [2] a tile's values are in its output
+  uint64_t* turn = o_done + 2;                  // [2][4] a warp's turn to take exponentials
+  float* q_mul = reinterpret_cast<float*>(smem + L::kOffMul);
   // pieces of 16 tokens that are there, of the last four tiles: two bits in each of four bytes (warps 8 to 11)
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kOffValid);
   Kv4Cursor& found = *reinterpret_cast<Kv4Cursor*>(smem + L::kOffCursor);
@@ -130,7 +146,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 128);
+      mbar_init(q_full + i, 32 * kPreLoaders);
+      mbar_init(q_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
       mbar_init(o_done + i, 1);
@@ -141,6 +158,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       mbar_init(v_full + i, 128);
       mbar_init(v_empty + i, 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(turn + i, 1);
     fence_mbar_init();
   }
   if (warp == 12) {
@@ -176,6 +194,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
     uint32_t s_phase = 0;  // token tiles so far
     int seen = 0;          // token tiles of the call, both row tiles'
+    uint32_t segments = 0, turns = 0;  // segments of this row tile; turns of this warp
     bool is_first = true, goes_on = false;
     for (;; is_first = false) {
       const int rows = at.seq.n * a.g.G - at.rt * kPreRows;  // of the segment, 256 at most count
@@ -184,48 +203,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       const bool there = tile * 128 + row_in < rows;
       const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
       const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
-      if (tile == 0 || rows > 128) {
-        float mul = 1.0f;
-        bool finite = true;
-        {
-          // the row as fp16 times a power of two that brings its largest element to [2^14, 2^15)
-          const unsigned short* src = a.q + static_cast<int64_t>(at.seq.row0 + i_tok) * a.q_row + static_cast<int64_t>(head) * a.q_head;
-          uint4 v[HD / 8];
-          uint32_t big = 0;
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i) {
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (there) v[i] = *reinterpret_cast<const uint4*>(src + 8 * i);
-          }
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i)
-            big = __vmaxu2(__vmaxu2(__vmaxu2(big, v[i].x & 0x7FFF7FFFu), __vmaxu2(v[i].y & 0x7FFF7FFFu, v[i].z & 0x7FFF7FFFu)),
-                           v[i].w & 0x7FFF7FFFu);
-          big = max(big & 0xFFFFu, big >> 16);
-          finite = big < 0x7F80u;
-          const int e = big > 0 && finite ? static_cast<int>(big >> 7) - 127 : 0;
-          const int up = max(min(14 - e, 100), -103);
-          float by = __int_as_float((up + 127) << 23);
-          mul = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
-          if (a.scale2 < 0.0f) by = -by;                    // (the maximum is taken of scores times |scale|)
-          if (a.scale2 == 0.0f || !finite) by = 0.0f, mul = 1.0f;
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i) {
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            uint32_t h[4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              // elements 2j, 2j + 1 and 2j + 4, 2j + 5; (x * 0 is NaN for an element that is not finite: such rows are made zero)
-              const uint32_t p = finite ? w[j] : 0u, q = finite ? w[j + 2] : 0u;
-              h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
-              h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
-            }
-            *reinterpret_cast<uint4*>(smem + L::kOffQ + tile * L::kOperand + (i >> 3) * L::kHalf + row_in * 128 +
-                                      (((i & 7) ^ (row_in & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(q_full + tile);
-        }
+      const bool two = rows > 128;
+      if (tile == 0 || two) {
         const int kv = min(at.seq.kv, a.c.capacity);
         const int p_row = at.seq.kv - at.seq.n + i_tok;
         const int hi = there ? min(p_row + 1, kv) : 0;                   // tokens lo ... hi - 1 and those below `first`
@@ -233,39 +212,53 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         const int first = a.m.window > 0 ? min(a.m.sinks, hi) : 0;
         float m = kKv4NoMax;
         float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        float mul = 0.0f;
+        bool finite = true;
         for (int j = 0; j < n_tiles && ok; ++j) {
           const int tok = at.span.tile(at.u0 + j) * kPreTile;
           ok = mbar_wait(s_full + tile, s_phase & 1, &s_abort, 42);
           tc_fence_after();
+          if (j == 0) {  // (written before the queries were handed to the products that have just finished)
+            mul = q_mul[(segments & 1) * kPreRows + tile * 128 + row_in];
+            finite = !isnan(mul);
+            mul = finite ? mul : 1.0f;
+            ++segments;
+          }
           const uint32_t got = valid[(seen + j) & 3];
           const bool whole = got == 0x03030303u && tok + kPreTile <= kv && tok + kPreTile <= at.span.p_lo + 1 &&
                              (a.m.window == 0 || tok > at.span.p_hi - a.m.window || tok + kPreTile <= a.m.sinks);
-          // Scores are read twice, 32 at a time, for the maximum and for the weights: 128 of them in registers would leave the
-          // converting warps too few.
-          auto hide = [&](uint32_t (&s)[32], int c0) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int t = tok + c0 + c;
-              const bool see = t < hi && (t >= lo || t < first) && ((got >> ((c0 >> 5) * 8 + (c >> 4))) & 1u);
-              if (!see) s[c] = 0xFF800000u;
-            }
-          };
-          uint32_t s[2][32];
+          auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u; };
+          // Scores are read twice, 64 at a time: first their maximum, and hidden ones go back as -inf.  (Held in registers, all 128
+          // take the code and the registers that keep the other warps from running: 1018 us against 806 for 8 prompts of 2048.)
+          uint32_t s[64];
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tmem_ld_x32(t_s, s[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 64) {
+            tmem_ld_x32(t_s + c, s);
+            tmem_ld_x32(t_s + c + 32, s + 32);
             tmem_ld_wait();
-            if (c < 3) tmem_ld_x32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
-            if (!whole) hide(s[c & 1], 32 * c);
+            if (!whole) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
+              for (int h = 0; h < 2; ++h) {
+                const int t0 = tok + c + 32 * h;
+                const uint32_t pieces = got >> (c / 4 + 8 * h);
+                const uint32_t see = below(hi - t0) & (~below(lo - t0) | below(first - t0)) &
+                                     ((pieces & 1u ? 0xFFFFu : 0u) | (pieces & 2u ? 0xFFFF0000u : 0u));
 #pragma unroll
-              for (int f = 0; f < 4; ++f)
-                top[f] = fmaxf(top[f], fmaxf(__uint_as_float(s[c & 1][e + f]), __uint_as_float(s[c & 1][e + f + 4])));
+                for (int e = 0; e < 32; ++e)
+                  if (!((see >> e) & 1u)) s[32 * h + e] = 0xFF800000u;
+                tmem_st_x32(t_s + c + 32 * h, s + 32 * h);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 64; e += 8)
+#pragma unroll
+              for (int f = 0; f < 4; ++f) top[f] = max3(top[f], __uint_as_float(s[e + f]), __uint_as_float(s[e + f + 4]));
           }
+          if (!whole) tmem_st_wait();
+          tmem_ld_x32(t_s, s);
+          tmem_ld_x32(t_s + 32, s + 32);
           const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
-          tmem_ld_x32(t_s, s[0]);
           if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
             const float to = fmaxf(m, high), by = pre_exp2(m - to);
             m = to;
@@ -274,7 +267,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             if (j > 0) {
               ok = ok && mbar_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the tile before is in O
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
                 uint32_t o[16];
                 tmem_ld_x16(t_o + c, o);
@@ -285,22 +278,30 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
               }
             }
           }
+          // The two row tiles take turns: side by side both would end at once, and the tensor cores would wait for both.
+          if (two) ok = ok && mbar_wait(turn + tile * 4 + (warp & 3), (turns & 1) ^ (tile ^ 1), &s_abort, 54);
           const float2 mul2 = make_float2(mul, mul), low = make_float2(-m, -m);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {  // 64 scores into 32 columns of weights, over scores that have been read
             tmem_ld_wait();
-            if (c < 3) tmem_ld_x32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
-            if (!whole) hide(s[c & 1], 32 * c);
-            uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 x =
-                  __ffma2_rn(make_float2(__uint_as_float(s[c & 1][2 * e]), __uint_as_float(s[c & 1][2 * e + 1])), mul2, low);
-              const float2 w = make_float2(pre_exp2(x.x), pre_exp2(x.y));
-              l2[e & 1] = __fadd2_rn(l2[e & 1], w);
-              p[e] = pre_half2(w.x, w.y);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t p[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float2 x = __ffma2_rn(
+                    make_float2(__uint_as_float(s[32 * h + 2 * e]), __uint_as_float(s[32 * h + 2 * e + 1])), mul2, low);
+                const float2 w = make_float2(pre_exp2(x.x), pre_exp2(x.y));
+                l2[e & 1] = __fadd2_rn(l2[e & 1], w);
+                p[e] = pre_half2(w.x, w.y);
+              }
+              if (c == 0) tmem_ld_x32(t_s + 64 + 32 * h, s + 32 * h);
+              pre_tmem_st_x16(t_s + c + 16 * h, p);
             }
-            pre_tmem_st_x16(t_s + 16 * c, p);  // (columns whose scores have been read)
+          }
+          if (two) {
+            if (lane == 0) mbar_arrive(turn + (tile ^ 1) * 4 + (warp & 3));
+            ++turns;
           }
           tmem_st_wait();
           tc_fence_before();
@@ -317,7 +318,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         if (!finite && l != 0.0f) by = __int_as_float(0x7FC00000);
         float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(kPreRows, HD);
         float* part_o = part + 2 * kPreRows + (tile * 128 + row_in) * HD;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];
           tmem_ld_x32(t_o + c, o);
@@ -374,104 +375,114 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     constexpr int kLoads = 32 / kStep;        // loads for the warp's 32 tokens
     const int w = warp - 8, q = lane % kLanes, in = lane / kLanes;
     const int P = 1 << a.c.page_shift;
-    struct Raw {
-      uint4 code[kLoads];
-      __half2 pair[kLoads];
-    } rk, rv;
     bool more = true;
     int u = at.u0;
-    uint32_t got = 0;               // this warp's two pieces of 16 tokens
-    const uint8_t* block[2];        // of the tile that is loaded next
+    uint32_t got = 0;               // this warp's two pieces of 16 tokens of the tile that is copied next
+    const uint8_t* block[2];
     int slot[2], left = 0;          // left: tokens of the tile from this warp's first one on
     auto seek = [&]() {
       while (more && u >= at.u1) {
         more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at);
         u = at.u0;
       }
-      got = 0;
       if (!more) return;
+      got = 0;
       const int tok = at.span.tile(u) * kPreTile + w * 32;
       left = min(at.seq.kv, a.c.capacity) - tok;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = tok + 16 * i;
-        int page = -1;
-        if (16 * i < left) page = a.c.table[at.b * a.c.table_stride + (t >> a.c.page_shift)];
-        if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.c.num_pages)) got |= 1u << i;
-        block[i] = a.c.pages + static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.c.page_stride) +
+        uint32_t page = 0xFFFFFFFFu;
+        if (16 * i < left) page = static_cast<uint32_t>(a.c.table[at.b * a.c.table_stride + (t >> a.c.page_shift)]);
+        const bool is = page < static_cast<uint32_t>(a.c.num_pages);
+        got |= is ? 1u << i : 0u;
+        block[i] = a.c.pages + static_cast<uint64_t>(is ? page : 0u) * static_cast<uint32_t>(a.c.page_stride) +
                    static_cast<int64_t>(at.h) * P * (HD + 8);
         slot[i] = t & (P - 1);
       }
       ++u;
     };
-    // tokens that are not there become zeros (their weights are zero, and zero times anything that a page may hold is not)
-    auto load = [&](Raw& r, bool values) {
+    // codes [32][HD / 2] and pairs [32] of the warp's tokens; pieces that are not there are left as they are in shared memory
+    uint8_t* const raw = smem + L::kOffRaw + w * 2 * L::kRaw;
+    auto copy = [&](bool values) {
+      if (more) {
+        const uint32_t dst = smem_u32(raw) + (values ? L::kRaw : 0);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int t = i * kStep + in, piece = (i * kStep) >> 4;  // (16 tokens are a multiple of kStep)
-        r.code[i] = make_uint4(0, 0, 0, 0);
-        r.pair[i] = __half2half2(__ushort_as_half(0));
-        if (((got >> piece) & 1u) && t < left) {
-          const int sl = slot[piece] + (t & 15);
-          r.code[i] = *reinterpret_cast<const uint4*>(block[piece] + (values ? P * (HD / 2) : 0) + sl * (HD / 2) + q * 16);
-          r.pair[i] = *reinterpret_cast<const __half2*>(block[piece] + P * HD + (values ? 4 * P : 0) + sl * 4);
+        for (int i = 0; i < 2; ++i) {
+          if ((got >> i) & 1u) {
+            const uint8_t* src = block[i] + (values ? P * (HD / 2) : 0) + slot[i] * (HD / 2) + lane * 16;
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) pre_cp_async_16(dst + i * 16 * (HD / 2) + e * 512 + lane * 16, src + e * 512);
+            if (lane < 4)
+              pre_cp_async_16(dst + 32 * (HD / 2) + i * 64 + lane * 16,
+                              block[i] + P * HD + (values ? 4 * P : 0) + slot[i] * 4 + lane * 16);
+          }
         }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto store = [&](const Raw& r, uint8_t* dst) {
-#pragma unroll
+    // keys of tile 0, values of tile 0, keys of tile 1 ...: one is converted while the next two are on the way
+    seek();
+    copy(false);
+    copy(true);
+    uint32_t got_now = got;
+    int left_now = left;
+    bool values = false, last = false;
+    for (uint32_t n = 0; ok && !last;) {
+      const int stage = n % kPreStages;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();
+      ok = mbar_wait((values ? v_empty : k_empty) + stage, ((n / kPreStages) & 1) ^ 1, &s_abort, 45);
+      // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
+      if (!values && lane == 0)
+        reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(got_now);
+      const uint8_t* from = raw + (values ? L::kRaw : 0);
+      // lanes of the second 64 elements take their words in the order 2 3 0 1: the eight lanes that store together hit eight
+      // different 16-byte columns
+      const int turned = q & 2;
+      uint8_t* to = smem + (values ? L::kOffV : L::kOffK) + stage * L::kOperand + (q >> 1) * L::kHalf;
+#pragma unroll 1
       for (int i = 0; i < kLoads; ++i) {
-        const int t = w * 32 + i * kStep + in;
-        const __half2 s = __low2half2(r.pair[i]), z = __high2half2(r.pair[i]);
-        uint32_t c[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
-        // lanes of the second 64 elements take their words in the order 2 3 0 1: the eight lanes that store together
-        // hit eight different 16-byte columns
-        const int turn = q & 2;
-        if (turn) {
-          uint32_t x = c[0];
-          c[0] = c[2], c[2] = x;
-          x = c[1];
-          c[1] = c[3], c[3] = x;
-        }
-        uint8_t* row = dst + (q >> 1) * L::kHalf + t * 128;
+        const int t = i * kStep + in;
+        const uint4 code = *reinterpret_cast<const uint4*>(from + t * (HD / 2) + q * 16);
+        __half2 pair = *reinterpret_cast<const __half2*>(from + 32 * (HD / 2) + t * 4);
+        // tokens that are not there become zeros: their weights are zero, and zero times what a slot may hold is not
+        if (t >= left_now || !((got_now >> (t >> 4)) & 1u)) pair = __half2half2(__ushort_as_half(0));
+        const __half2 sc = __low2half2(pair), ze = __high2half2(pair);
+        const uint32_t c[4] = {turned ? code.z : code.x, turned ? code.w : code.y, turned ? code.x : code.z,
+                               turned ? code.y : code.w};
+        uint8_t* row = to + (w * 32 + t) * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint4*>(row + (((((q & 1) << 2) + (e ^ turn)) ^ (t & 7)) << 4)) = pre_expand(c[e], s, z);
+          *reinterpret_cast<uint4*>(row + (((((q & 1) << 2) + (e ^ turned)) ^ (t & 7)) << 4)) = pre_expand(c[e], sc, ze);
       }
       fence_proxy_async_smem();
-    };
-    seek();
-    load(rk, false);
-    load(rv, true);
-    for (uint32_t n = 0; more && ok; ++n) {
-      const int stage = n % kPreStages;
-      const uint32_t parity = ((n / kPreStages) & 1) ^ 1;
-      const uint32_t mine = got;
-      ok = mbar_wait(k_empty + stage, parity, &s_abort, 45);
-      // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
-      if (lane == 0) reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(mine);
-      store(rk, smem + L::kOffK + stage * L::kOperand);
-      mbar_arrive(k_full + stage);
-      const Raw now = rv;
-      seek();
-      if (more) load(rk, false);
-      ok = ok && mbar_wait(v_empty + stage, parity, &s_abort, 46);
-      store(now, smem + L::kOffV + stage * L::kOperand);
-      mbar_arrive(v_full + stage);
-      if (more) load(rv, true);
+      mbar_arrive((values ? v_full : k_full) + stage);
+      __syncwarp();  // every lane has read the codes
+      if (!values) seek();  // the tile behind this one
+      copy(values);
+      if (values) {
+        last = !more;
+        got_now = got;
+        left_now = left;
+        ++n;
+      }
+      values = !values;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp == 12) {
     // ------------------------------------------------------------------------------------------------ products
     if (elect_one()) {
       constexpr uint32_t kIdescS = pre_idesc(128, 128, false), kIdescO = pre_idesc(128, HD, true);
       uint32_t q_phase = 0, q1_phase = 0, p_phase0 = 0, p_phase1 = 0, n = 0;  // n: token tiles so far
-      auto scores = [&](int tile, uint32_t stage) {
+      auto scores = [&](int tile, uint32_t stage, bool last) {
         const uint32_t qa = base + L::kOffQ + tile * L::kOperand, ka = base + L::kOffK + stage * L::kOperand;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
           pre_mma_ss(tmem + tile * 128, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
                      umma_desc_k_sw128(ka + (k >> 2) * L::kHalf + (k & 3) * 32), kIdescS, k > 0);
         umma_commit(s_full + tile);
+        if (last) umma_commit(q_empty + tile);
       };
       auto values = [&](int tile, uint32_t stage, bool add) {
         const uint32_t va = base + L::kOffV + stage * L::kOperand;
@@ -493,8 +504,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         ok = ok && mbar_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
         if (!ok) break;
         tc_fence_after();
-        scores(0, n % kPreStages);
-        if (two) scores(1, n % kPreStages);
+        scores(0, n % kPreStages, n_tiles == 1);
+        if (two) scores(1, n % kPreStages, n_tiles == 1);
         umma_commit(k_empty + n % kPreStages);
         for (int j = 0; j < n_tiles && ok; ++j, ++n) {
           const uint32_t stage = n % kPreStages, next = (n + 1) % kPreStages;
@@ -509,7 +520,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             ok = mbar_wait(k_full + next, ((n + 1) / kPreStages) & 1, &s_abort, 52);
             if (!ok) break;
             tc_fence_after();
-            scores(0, next);
+            scores(0, next, j + 2 == n_tiles);
           }
           if (two) {
             ok = mbar_wait(p_full + 1, p_phase1 & 1, &s_abort, 53);
@@ -520,7 +531,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           }
           umma_commit(v_empty + stage);
           if (!last) {
-            if (two) scores(1, next);
+            if (two) scores(1, next, j + 2 == n_tiles);
             umma_commit(k_empty + next);
           }
         }
@@ -528,6 +539,64 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       }
     }
     __syncwarp();
+  } else {
+    // ------------------------------------------------------------------------------------------------ queries
+    // A row as fp16 times a power of two that brings its largest element to [2^14, 2^15), HD / 8 lanes a row.
+    // The rows come in by asynchronous copies, all of a row tile at once, and every lane converts the 16 bytes that it copied.
+    constexpr int kRowLanes = HD / 8, kRowsAtOnce = 32 / kRowLanes;
+    const int w = warp - 13, chunk = lane % kRowLanes, row0 = w * kRowsAtOnce + lane / kRowLanes;
+    uint32_t uses[2] = {0, 0};
+    for (;;) {
+      const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
+#pragma unroll 1
+      for (int tile = 0; tile < (rows > 128 ? 2 : 1); ++tile) {
+        const uint32_t use = uses[tile]++;
+        ok = ok && mbar_wait(q_empty + tile, (use & 1) ^ 1, &s_abort, 55);
+        uint8_t* const dst = smem + L::kOffQ + tile * L::kOperand + (chunk >> 3) * L::kHalf;
+        auto place = [&](int row) { return dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
+#pragma unroll 1
+        for (int row = row0; row < 128; row += kPreLoaders * kRowsAtOnce) {
+          const bool there = tile * 128 + row < rows;
+          const int r = at.rt * kPreRows + tile * 128 + row, i_tok = there ? a.g.by(r) : 0;
+          const int head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
+          pre_cp_async_16(smem_u32(place(row)),
+                          a.q + static_cast<int64_t>(at.seq.row0 + i_tok) * a.q_row + static_cast<int64_t>(head) * a.q_head +
+                              8 * chunk,
+                          there ? 16 : 0);
+        }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+        float* mul_out = q_mul + (use & 1) * kPreRows + tile * 128;
+#pragma unroll 2
+        for (int row = row0; row < 128; row += kPreLoaders * kRowsAtOnce) {
+          uint4* const at_row = reinterpret_cast<uint4*>(place(row));
+          const uint4 v = *at_row;
+          uint32_t big = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+#pragma unroll
+          for (int d = 1; d < kRowLanes; d <<= 1) big = __vmaxu2(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+          big = max(big & 0xFFFFu, big >> 16);
+          const bool finite = big < 0x7F80u;  // no infinity and no NaN; rows that are not finite are made zero here
+          const int e = big > 0 && finite ? static_cast<int>(big >> 7) - 127 : 0;
+          const int up = max(min(14 - e, 100), -103);
+          float by = __int_as_float((up + 127) << 23);
+          float mul = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
+          if (a.scale2 < 0.0f) by = -by;  // (the maximum is taken of scores times |scale|)
+          if (a.scale2 == 0.0f) by = 0.0f, mul = 1.0f;
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {  // elements 2j, 2j + 1 and 2j + 4, 2j + 5
+            const uint32_t p = finite ? x[j] : 0u, q = finite ? x[j + 2] : 0u;
+            h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
+            h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
+          }
+          *at_row = make_uint4(h[0], h[1], h[2], h[3]);
+          if (chunk == 0) mul_out[row] = finite ? mul : __int_as_float(0x7FC00000);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full + tile);
+      }
+      if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
+    }
   }
   // every product has been waited for by the softmax of its row tile (or a wait ran out)
   tc_fence_before();
