@@ -33,7 +33,7 @@ struct PreSmem {
   static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
   static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
   static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
-  static constexpr int kBars = 4 + 4 * kPreStages + 6 + 8;
+  static constexpr int kBars = 4 + 4 * kPreStages + 6;
   static constexpr int kOffValid = kOffBar + kBars * 8;
   static constexpr int kOffMul = kOffValid + 4 * 4;            // [2][256] what a row's scores have to be multiplied with
   static constexpr int kOffCursor = kOffMul + 2 * kPreRows * 4;
@@ -99,6 +99,30 @@ __device__ __forceinline__ uint32_t pre_bf16x2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// mbar_wait with a hint of how long the wait may sleep: sixteen warps share the issue slots, most of them waiting.
+__device__ __forceinline__ bool pre_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int site) {
+  auto ready = [&]() {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\nselp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+  };
+  if (ready()) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+      if (ready()) return true;
+    if (*abort_flag != 0) return false;
+    if (clock64() - t0 > (1ll << 31)) {
+      *abort_flag = site;
+      return false;
+    }
+  }
+}
 // eight codes -> fp16 c * scale + zero, elements 0 4 1 5 2 6 3 7
 __device__ __forceinline__ uint4 pre_expand(uint32_t w, __half2 s, __half2 z) {
   const __half2 k1024 = __half2half2(__ushort_as_half(0x6400)), k16th = __half2half2(__ushort_as_half(0x2C00)),
@@ -136,7 +160,6 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   uint64_t* s_full = v_empty + kPreStages;      // [2] scores of a row tile are in tensor memory
   uint64_t* p_full = s_full + 2;                // [2] its weights are
   uint64_t* o_done = p_full + 2;                // [2] a tile's values are in its output
-  uint64_t* turn = o_done + 2;                  // [2][4] a warp's turn to take exponentials
   float* q_mul = reinterpret_cast<float*>(smem + L::kOffMul);
   // pieces of 16 tokens that are there, of the last four tiles: two bits in each of four bytes (warps 8 to 11)
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kOffValid);
@@ -158,7 +181,6 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       mbar_init(v_full + i, 128);
       mbar_init(v_empty + i, 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(turn + i, 1);
     fence_mbar_init();
   }
   if (warp == 12) {
@@ -194,7 +216,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
     uint32_t s_phase = 0;  // token tiles so far
     int seen = 0;          // token tiles of the call, both row tiles'
-    uint32_t segments = 0, turns = 0;  // segments of this row tile; turns of this warp
+    uint32_t segments = 0;  // segments of this row tile
     bool is_first = true, goes_on = false;
     for (;; is_first = false) {
       const int rows = at.seq.n * a.g.G - at.rt * kPreRows;  // of the segment, 256 at most count
@@ -203,20 +225,19 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       const bool there = tile * 128 + row_in < rows;
       const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
       const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
-      const bool two = rows > 128;
-      if (tile == 0 || two) {
+      if (tile == 0 || rows > 128) {
         const int kv = min(at.seq.kv, a.c.capacity);
         const int p_row = at.seq.kv - at.seq.n + i_tok;
         const int hi = there ? min(p_row + 1, kv) : 0;                   // tokens lo ... hi - 1 and those below `first`
         const int lo = a.m.window > 0 ? p_row - a.m.window + 1 : 0;
         const int first = a.m.window > 0 ? min(a.m.sinks, hi) : 0;
         float m = kKv4NoMax;
-        float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        float2 l2 = make_float2(0.0f, 0.0f);
         float mul = 0.0f;
         bool finite = true;
         for (int j = 0; j < n_tiles && ok; ++j) {
           const int tok = at.span.tile(at.u0 + j) * kPreTile;
-          ok = mbar_wait(s_full + tile, s_phase & 1, &s_abort, 42);
+          ok = pre_wait(s_full + tile, s_phase & 1, &s_abort, 42);
           tc_fence_after();
           if (j == 0) {  // (written before the queries were handed to the products that have just finished)
             mul = q_mul[(segments & 1) * kPreRows + tile * 128 + row_in];
@@ -262,10 +283,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
             const float to = fmaxf(m, high), by = pre_exp2(m - to);
             m = to;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) l2[e].x *= by, l2[e].y *= by;
+            l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
-              ok = ok && mbar_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the tile before is in O
+              ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the tile before is in O
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -278,30 +298,36 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
               }
             }
           }
-          // The two row tiles take turns: side by side both would end at once, and the tensor cores would wait for both.
-          if (two) ok = ok && mbar_wait(turn + tile * 4 + (warp & 3), (turns & 1) ^ (tile ^ 1), &s_abort, 54);
           const float2 mul2 = make_float2(mul, mul), low = make_float2(-m, -m);
+          // 64 scores into 32 columns of weights, over scores that have been read.  Sixteen at a time; sums and stores are a
+          // batch behind, or they would wait for every exponential: 662 cycles for 64 scores of a warp by itself, 1097 with sums
+          // in the order of the scores.
 #pragma unroll 1
-          for (int c = 0; c < 64; c += 32) {  // 64 scores into 32 columns of weights, over scores that have been read
+          for (int c = 0; c < 64; c += 32) {
             tmem_ld_wait();
+            float2 w[2][8];
+            uint32_t p[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t p[16];
+            for (int b = 0; b < 5; ++b) {
+              if (b < 4) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float2 x = __ffma2_rn(
-                    make_float2(__uint_as_float(s[32 * h + 2 * e]), __uint_as_float(s[32 * h + 2 * e + 1])), mul2, low);
-                const float2 w = make_float2(pre_exp2(x.x), pre_exp2(x.y));
-                l2[e & 1] = __fadd2_rn(l2[e & 1], w);
-                p[e] = pre_half2(w.x, w.y);
+                for (int e = 0; e < 8; ++e) {
+                  const float2 x = __ffma2_rn(
+                      make_float2(__uint_as_float(s[16 * b + 2 * e]), __uint_as_float(s[16 * b + 2 * e + 1])), mul2, low);
+                  w[b & 1][e] = make_float2(pre_exp2(x.x), pre_exp2(x.y));
+                }
               }
-              if (c == 0) tmem_ld_x32(t_s + 64 + 32 * h, s + 32 * h);
-              pre_tmem_st_x16(t_s + c + 16 * h, p);
+              if (b == 2 && c == 0) tmem_ld_x32(t_s + 64, s);
+              if (b > 0) {
+                const float2(&v)[8] = w[(b - 1) & 1];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[8 * ((b - 1) & 1) + e] = pre_half2(v[e].x, v[e].y);
+                l2 = __fadd2_rn(l2, __fadd2_rn(__fadd2_rn(__fadd2_rn(v[0], v[1]), __fadd2_rn(v[2], v[3])),
+                                               __fadd2_rn(__fadd2_rn(v[4], v[5]), __fadd2_rn(v[6], v[7]))));
+                if (((b - 1) & 1) == 1) pre_tmem_st_x16(t_s + c + 8 * (b - 2), p);
+              }
             }
-          }
-          if (two) {
-            if (lane == 0) mbar_arrive(turn + (tile ^ 1) * 4 + (warp & 3));
-            ++turns;
+            if (c == 0) tmem_ld_x32(t_s + 96, s + 32);
           }
           tmem_st_wait();
           tc_fence_before();
@@ -309,8 +335,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           ++s_phase;
         }
         // output of the row
-        const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
-        ok = ok && mbar_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 44);
+        const float l = l2.x + l2.y;
+        ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 44);
         tc_fence_after();
         const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
         // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
@@ -323,27 +349,47 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           uint32_t o[32];
           tmem_ld_x32(t_o + c, o);
           tmem_ld_wait();
-          if (there && ok) {
 #pragma unroll
-            for (int g = 0; g < 32; g += 8) {
-              float v[8];  // elements in their own order
+          for (int g = 0; g < 32; g += 8) {  // elements into their own order
+            float v[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                v[e] = __uint_as_float(o[g + 2 * e]) * by;
-                v[e + 4] = __uint_as_float(o[g + 2 * e + 1]) * by;
-              }
-              if (l == 0.0f) {
+            for (int e = 0; e < 4; ++e) {
+              v[e] = __uint_as_float(o[g + 2 * e]) * by;
+              v[e + 4] = __uint_as_float(o[g + 2 * e + 1]) * by;
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-              }
-              if (whole_segment) {
-                *reinterpret_cast<uint4*>(a.out + out_at + c + g) =
-                    make_uint4(pre_bf16x2(v[0], v[1]), pre_bf16x2(v[2], v[3]), pre_bf16x2(v[4], v[5]), pre_bf16x2(v[6], v[7]));
-              } else {
-                *reinterpret_cast<float4*>(part_o + c + g) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4*>(part_o + c + g + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            for (int e = 0; e < 8; ++e) o[g + e] = __float_as_uint(l == 0.0f ? 0.0f : v[e]);
+          }
+          if (whole_segment) {
+            // four lanes exchange their 64 bytes so that they store one row together, then the next
+            uint4 x[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float* v = reinterpret_cast<const float*>(o + 8 * g);
+              x[g] = make_uint4(pre_bf16x2(v[0], v[1]), pre_bf16x2(v[2], v[3]), pre_bf16x2(v[4], v[5]), pre_bf16x2(v[6], v[7]));
+            }
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                if (g & d) continue;
+                const bool up = lane & d;  // gives x[g], keeps x[g + d]
+                const uint4 give = up ? x[g] : x[g + d];
+                const uint4 take = make_uint4(__shfl_xor_sync(0xFFFFFFFFu, give.x, d), __shfl_xor_sync(0xFFFFFFFFu, give.y, d),
+                                              __shfl_xor_sync(0xFFFFFFFFu, give.z, d), __shfl_xor_sync(0xFFFFFFFFu, give.w, d));
+                if (up) x[g] = take;
+                else x[g + d] = take;
               }
             }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {  // 16 bytes lane % 4 of the row of lane (lane & ~3) + g
+              const long long row_at = __shfl_sync(0xFFFFFFFFu, there ? static_cast<long long>(out_at) : -1ll, (lane & ~3) + g);
+              if (row_at >= 0 && ok) *reinterpret_cast<uint4*>(a.out + row_at + c + 8 * (lane & 3)) = x[g];
+            }
+          } else if (there && ok) {
+#pragma unroll
+            for (int g = 0; g < 32; g += 4)
+              *reinterpret_cast<uint4*>(part_o + c + g) = make_uint4(o[g], o[g + 1], o[g + 2], o[g + 3]);
           }
         }
         if (!whole_segment && there) {
@@ -375,32 +421,45 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     constexpr int kLoads = 32 / kStep;        // loads for the warp's 32 tokens
     const int w = warp - 8, q = lane % kLanes, in = lane / kLanes;
     const int P = 1 << a.c.page_shift;
-    bool more = true;
-    int u = at.u0;
-    uint32_t got = 0;               // this warp's two pieces of 16 tokens of the tile that is copied next
+    // The tile that is copied next (`got`: this warp's two pieces of 16 tokens that are there, `left`: tokens of the tile from
+    // this warp's first one on), and the page numbers of the one behind it, which are on their way.
+    bool more = true, coming = true;
+    int u = at.u0, h_next = 0, tok_next = 0, left_next = 0;
+    uint32_t page_next[2];
+    uint32_t got = 0;
     const uint8_t* block[2];
-    int slot[2], left = 0;          // left: tokens of the tile from this warp's first one on
-    auto seek = [&]() {
-      while (more && u >= at.u1) {
-        more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at);
+    int slot[2], left = 0;
+    auto look_up = [&]() {
+      while (coming && u >= at.u1) {
+        coming = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at);
         u = at.u0;
       }
-      if (!more) return;
-      got = 0;
-      const int tok = at.span.tile(u) * kPreTile + w * 32;
-      left = min(at.seq.kv, a.c.capacity) - tok;
+      if (!coming) return;
+      tok_next = at.span.tile(u) * kPreTile + w * 32;
+      left_next = min(at.seq.kv, a.c.capacity) - tok_next;
+      h_next = at.h;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int t = tok + 16 * i;
-        uint32_t page = 0xFFFFFFFFu;
-        if (16 * i < left) page = static_cast<uint32_t>(a.c.table[at.b * a.c.table_stride + (t >> a.c.page_shift)]);
-        const bool is = page < static_cast<uint32_t>(a.c.num_pages);
-        got |= is ? 1u << i : 0u;
-        block[i] = a.c.pages + static_cast<uint64_t>(is ? page : 0u) * static_cast<uint32_t>(a.c.page_stride) +
-                   static_cast<int64_t>(at.h) * P * (HD + 8);
-        slot[i] = t & (P - 1);
+        page_next[i] = 0xFFFFFFFFu;
+        if (16 * i < left_next)
+          page_next[i] = static_cast<uint32_t>(a.c.table[at.b * a.c.table_stride + ((tok_next + 16 * i) >> a.c.page_shift)]);
       }
       ++u;
+    };
+    auto seek = [&]() {
+      more = coming;
+      if (!more) return;
+      got = 0;
+      left = left_next;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool is = page_next[i] < static_cast<uint32_t>(a.c.num_pages);
+        got |= is ? 1u << i : 0u;
+        block[i] = a.c.pages + static_cast<uint64_t>(is ? page_next[i] : 0u) * static_cast<uint32_t>(a.c.page_stride) +
+                   static_cast<int64_t>(h_next) * P * (HD + 8);
+        slot[i] = (tok_next + 16 * i) & (P - 1);
+      }
+      look_up();
     };
     // codes [32][HD / 2] and pairs [32] of the warp's tokens; pieces that are not there are left as they are in shared memory
     uint8_t* const raw = smem + L::kOffRaw + w * 2 * L::kRaw;
@@ -422,6 +481,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // keys of tile 0, values of tile 0, keys of tile 1 ...: one is converted while the next two are on the way
+    look_up();
     seek();
     copy(false);
     copy(true);
@@ -432,7 +492,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       const int stage = n % kPreStages;
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();
-      ok = mbar_wait((values ? v_empty : k_empty) + stage, ((n / kPreStages) & 1) ^ 1, &s_abort, 45);
+      ok = pre_wait((values ? v_empty : k_empty) + stage, ((n / kPreStages) & 1) ^ 1, &s_abort, 45);
       // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
       if (!values && lane == 0)
         reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(got_now);
@@ -441,16 +501,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       // different 16-byte columns
       const int turned = q & 2;
       uint8_t* to = smem + (values ? L::kOffV : L::kOffK) + stage * L::kOperand + (q >> 1) * L::kHalf;
-#pragma unroll 1
+#pragma unroll 2
       for (int i = 0; i < kLoads; ++i) {
         const int t = i * kStep + in;
-        const uint4 code = *reinterpret_cast<const uint4*>(from + t * (HD / 2) + q * 16);
+        const uint8_t* src = from + t * (HD / 2) + q * 16;
+        const uint2 c01 = *reinterpret_cast<const uint2*>(src + 4 * turned), c23 = *reinterpret_cast<const uint2*>(src + (8 - 4 * turned));
         __half2 pair = *reinterpret_cast<const __half2*>(from + 32 * (HD / 2) + t * 4);
         // tokens that are not there become zeros: their weights are zero, and zero times what a slot may hold is not
         if (t >= left_now || !((got_now >> (t >> 4)) & 1u)) pair = __half2half2(__ushort_as_half(0));
         const __half2 sc = __low2half2(pair), ze = __high2half2(pair);
-        const uint32_t c[4] = {turned ? code.z : code.x, turned ? code.w : code.y, turned ? code.x : code.z,
-                               turned ? code.y : code.w};
+        const uint32_t c[4] = {c01.x, c01.y, c23.x, c23.y};
         uint8_t* row = to + (w * 32 + t) * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -495,13 +555,13 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       for (;;) {
         const int rows = at.seq.n * a.g.G - at.rt * kPreRows, n_tiles = at.u1 - at.u0;
         const bool two = rows > 128;
-        ok = ok && mbar_wait(q_full, q_phase & 1, &s_abort, 47);
+        ok = ok && pre_wait(q_full, q_phase & 1, &s_abort, 47);
         ++q_phase;
         if (two) {
-          ok = ok && mbar_wait(q_full + 1, q1_phase & 1, &s_abort, 48);
+          ok = ok && pre_wait(q_full + 1, q1_phase & 1, &s_abort, 48);
           ++q1_phase;
         }
-        ok = ok && mbar_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
+        ok = ok && pre_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
         if (!ok) break;
         tc_fence_after();
         scores(0, n % kPreStages, n_tiles == 1);
@@ -510,20 +570,20 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         for (int j = 0; j < n_tiles && ok; ++j, ++n) {
           const uint32_t stage = n % kPreStages, next = (n + 1) % kPreStages;
           const bool last = j + 1 == n_tiles;
-          ok = mbar_wait(v_full + stage, (n / kPreStages) & 1, &s_abort, 50);
-          ok = ok && mbar_wait(p_full, p_phase0 & 1, &s_abort, 51);
+          ok = pre_wait(v_full + stage, (n / kPreStages) & 1, &s_abort, 50);
+          ok = ok && pre_wait(p_full, p_phase0 & 1, &s_abort, 51);
           ++p_phase0;
           tc_fence_after();
           if (!ok) break;
           values(0, stage, j > 0);
           if (!last) {
-            ok = mbar_wait(k_full + next, ((n + 1) / kPreStages) & 1, &s_abort, 52);
+            ok = pre_wait(k_full + next, ((n + 1) / kPreStages) & 1, &s_abort, 52);
             if (!ok) break;
             tc_fence_after();
             scores(0, next, j + 2 == n_tiles);
           }
           if (two) {
-            ok = mbar_wait(p_full + 1, p_phase1 & 1, &s_abort, 53);
+            ok = pre_wait(p_full + 1, p_phase1 & 1, &s_abort, 53);
             ++p_phase1;
             if (!ok) break;
             tc_fence_after();
@@ -543,54 +603,73 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     // ------------------------------------------------------------------------------------------------ queries
     // A row as fp16 times a power of two that brings its largest element to [2^14, 2^15), HD / 8 lanes a row.
     // The rows come in by asynchronous copies, all of a row tile at once, and every lane converts the 16 bytes that it copied.
-    constexpr int kRowLanes = HD / 8, kRowsAtOnce = 32 / kRowLanes;
-    const int w = warp - 13, chunk = lane % kRowLanes, row0 = w * kRowsAtOnce + lane / kRowLanes;
+    constexpr int kRowLanes = HD / 16, kRowsAtOnce = 32 / kRowLanes, kStep = kPreLoaders * kRowsAtOnce;
+    const int w = warp - 13, l = lane % kRowLanes, row0 = w * kRowsAtOnce + lane / kRowLanes;
     uint32_t uses[2] = {0, 0};
     for (;;) {
       const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
 #pragma unroll 1
       for (int tile = 0; tile < (rows > 128 ? 2 : 1); ++tile) {
         const uint32_t use = uses[tile]++;
-        ok = ok && mbar_wait(q_empty + tile, (use & 1) ^ 1, &s_abort, 55);
-        uint8_t* const dst = smem + L::kOffQ + tile * L::kOperand + (chunk >> 3) * L::kHalf;
-        auto place = [&](int row) { return dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
+        ok = ok && pre_wait(q_empty + tile, (use & 1) ^ 1, &s_abort, 55);
+        // 16-byte columns 2l and 2l + 1 of a row
+        uint8_t* const dst = smem + L::kOffQ + tile * L::kOperand + (l >> 2) * L::kHalf;
+        auto place = [&](int row, int c) { return dst + row * 128 + (((((2 * l) & 7) + c) ^ (row & 7)) << 4); };
 #pragma unroll 1
-        for (int row = row0; row < 128; row += kPreLoaders * kRowsAtOnce) {
+        for (int row = row0; row < 128; row += kStep) {
           const bool there = tile * 128 + row < rows;
           const int r = at.rt * kPreRows + tile * 128 + row, i_tok = there ? a.g.by(r) : 0;
           const int head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
-          pre_cp_async_16(smem_u32(place(row)),
-                          a.q + static_cast<int64_t>(at.seq.row0 + i_tok) * a.q_row + static_cast<int64_t>(head) * a.q_head +
-                              8 * chunk,
-                          there ? 16 : 0);
+          const unsigned short* src =
+              a.q + static_cast<int64_t>(at.seq.row0 + i_tok) * a.q_row + static_cast<int64_t>(head) * a.q_head + 16 * l;
+          pre_cp_async_16(smem_u32(place(row, 0)), src, there ? 16 : 0);
+          pre_cp_async_16(smem_u32(place(row, 1)), src + 8, there ? 16 : 0);
         }
         asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         float* mul_out = q_mul + (use & 1) * kPreRows + tile * 128;
-#pragma unroll 2
-        for (int row = row0; row < 128; row += kPreLoaders * kRowsAtOnce) {
-          uint4* const at_row = reinterpret_cast<uint4*>(place(row));
-          const uint4 v = *at_row;
-          uint32_t big = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+#pragma unroll 1
+        for (int base_row = w * kRowsAtOnce; base_row < 128; base_row += kStep) {
+          const int row = base_row + lane / kRowLanes;
+          const bool in = row < 128;  // (the last round of HD 128 has rows for some of the warp's lanes only)
+          uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+          if (in) v[0] = *reinterpret_cast<const uint4*>(place(row, 0)), v[1] = *reinterpret_cast<const uint4*>(place(row, 1));
+          uint32_t big = 0;
 #pragma unroll
-          for (int d = 1; d < kRowLanes; d <<= 1) big = __vmaxu2(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+          for (int i = 0; i < 2; ++i)
+            big = __vmaxu2(big, __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
+                                         __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
           big = max(big & 0xFFFFu, big >> 16);
-          const bool finite = big < 0x7F80u;  // no infinity and no NaN; rows that are not finite are made zero here
-          const int e = big > 0 && finite ? static_cast<int>(big >> 7) - 127 : 0;
-          const int up = max(min(14 - e, 100), -103);
-          float by = __int_as_float((up + 127) << 23);
-          float mul = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
+          // Ordinary rows, largest element in [2^-10, 2^15), are fp16 as they are (what lies below 2^-14 of them is off by 2^-25
+          // at most); if one of the warp's rows is not, the factors of all of them are looked up.
+          const uint32_t small = __ballot_sync(0xFFFFFFFFu, big < 0x3A80u);
+          constexpr uint32_t kRowMask = (1u << kRowLanes) - 1u;
+          const bool odd = big >= 0x4700u || ((small >> (lane & ~(kRowLanes - 1))) & kRowMask) == kRowMask;
+          bool finite = true;
+          float by = 1.0f, mul = fmaxf(fabsf(a.scale2), 1.2e-38f);
+          if (__any_sync(0xFFFFFFFFu, odd)) {
+#pragma unroll
+            for (int d = 1; d < kRowLanes; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+            finite = big < 0x7F80u;  // no infinity and no NaN; rows that are not finite are made zero here
+            const int e = big > 0 && finite ? static_cast<int>(big >> 7) - 127 : 0;
+            const int up = max(min(14 - e, 100), -103);
+            by = __int_as_float((up + 127) << 23);
+            mul = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
+          }
           if (a.scale2 < 0.0f) by = -by;  // (the maximum is taken of scores times |scale|)
           if (a.scale2 == 0.0f) by = 0.0f, mul = 1.0f;
-          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-          uint32_t h[4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {  // elements 2j, 2j + 1 and 2j + 4, 2j + 5
-            const uint32_t p = finite ? x[j] : 0u, q = finite ? x[j + 2] : 0u;
-            h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
-            h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {  // elements 2j, 2j + 1 and 2j + 4, 2j + 5
+              const uint32_t p = finite ? x[j] : 0u, q = finite ? x[j + 2] : 0u;
+              h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
+              h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
+            }
+            if (in) *reinterpret_cast<uint4*>(place(row, i)) = make_uint4(h[0], h[1], h[2], h[3]);
           }
-          *at_row = make_uint4(h[0], h[1], h[2], h[3]);
-          if (chunk == 0) mul_out[row] = finite ? mul : __int_as_float(0x7FC00000);
+          if (in && l == 0) mul_out[row] = finite ? mul : __int_as_float(0x7FC00000);
         }
         fence_proxy_async_smem();
         mbar_arrive(q_full + tile);
