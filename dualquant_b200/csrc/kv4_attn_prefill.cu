@@ -7,9 +7,8 @@
 //   warps 8-11       codes from the pages to fp16 keys and values (fma(c, scale, zero), one rounding) in shared memory
 //   warp 12          issues the products: S = Q K' (both from shared memory), O += P V (P from tensor memory)
 //   warps 13-15      queries of the next segment into shared memory as soon as its predecessor's last scores are computed
-// While the tensor cores work for one row tile, the exponentials of the other are taken: 128 x 128 products of depth 128 take
-// 512 cycles, twice a row tile and token tile, and so do 128 x 128 exponentials at 16 a cycle, so the two pipes would be busy
-// alike.  Tensor memory (512 columns): S0, S1 (the weights take the first half of their scores' columns), O0, O1.
+// Softmax goes by groups of 64 tokens, whose scores a thread holds in registers.  Tensor memory (512 columns): two buffers of 64
+// scores for each row tile (weights take the first half of their scores' columns) and the outputs of both.
 //
 // Operands are fp16: a key or value of the cache is c * scale + zero with fp16 scale and zero, and 11 bits keep that to 2^-11
 // where bf16 would give 2^-8; queries (bf16) are exact in fp16 times a power of two of their row; weights lie in [0, 2^8].
@@ -33,7 +32,7 @@ struct PreSmem {
   static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
   static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
   static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
-  static constexpr int kBars = 4 + 4 * kPreStages + 6;
+  static constexpr int kBars = 4 + 4 * kPreStages + 10;
   static constexpr int kOffValid = kOffBar + kBars * 8;
   static constexpr int kOffMul = kOffValid + 4 * 4;            // [2][256] what a row's scores have to be multiplied with
   static constexpr int kOffCursor = kOffMul + 2 * kPreRows * 4;
@@ -141,6 +140,13 @@ __device__ __forceinline__ uint4 pre_expand(uint32_t w, __half2 s, __half2 z) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// Groups of 64 tokens of a segment's share of tiles: the last tile's second group may lie behind all that the rows see.
+__device__ __forceinline__ int pre_groups(const Kv4Batch& c, const Kv4Cursor& k) {
+  const int n = 2 * (k.u1 - k.u0);
+  const int hi = min(min(k.span.p_hi + 1, k.seq.kv), c.capacity);
+  return k.u1 == k.span.count && hi <= k.span.tile(k.u1 - 1) * kPreTile + 64 ? n - 1 : n;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kPreThreads, 1)
 kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
@@ -157,9 +163,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   uint64_t* k_empty = k_full + kPreStages;
   uint64_t* v_full = k_empty + kPreStages;
   uint64_t* v_empty = v_full + kPreStages;
-  uint64_t* s_full = v_empty + kPreStages;      // [2] scores of a row tile are in tensor memory
-  uint64_t* p_full = s_full + 2;                // [2] its weights are
-  uint64_t* o_done = p_full + 2;                // [2] a tile's values are in its output
+  uint64_t* s_full = v_empty + kPreStages;      // [row tile][buffer] scores are in tensor memory
+  uint64_t* p_full = s_full + 4;                // [row tile][buffer] weights are
+  uint64_t* o_done = p_full + 4;                // [row tile] 64 tokens' values are in its output
   float* q_mul = reinterpret_cast<float*>(smem + L::kOffMul);
   // pieces of 16 tokens that are there, of the last four tiles: two bits in each of four bytes (warps 8 to 11)
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kOffValid);
@@ -171,9 +177,11 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 32 * kPreLoaders);
       mbar_init(q_empty + i, 1);
+      mbar_init(o_done + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
-      mbar_init(o_done + i, 1);
     }
     for (int i = 0; i < kPreStages; ++i) {
       mbar_init(k_full + i, 128);
@@ -214,13 +222,13 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const int tile = warp >> 2, row_in = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes, in the upper half of an address
     const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
-    uint32_t s_phase = 0;  // token tiles so far
+    uint32_t s_phase = 0;  // groups of 64 tokens so far
     int seen = 0;          // token tiles of the call, both row tiles'
     uint32_t segments = 0;  // segments of this row tile
     bool is_first = true, goes_on = false;
     for (;; is_first = false) {
       const int rows = at.seq.n * a.g.G - at.rt * kPreRows;  // of the segment, 256 at most count
-      const int n_tiles = at.u1 - at.u0;
+      const int n_groups = pre_groups(a.c, at);
       const int r = at.rt * kPreRows + tile * 128 + row_in;
       const bool there = tile * 128 + row_in < rows;
       const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
@@ -235,9 +243,10 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         float2 l2 = make_float2(0.0f, 0.0f);
         float mul = 0.0f;
         bool finite = true;
-        for (int j = 0; j < n_tiles && ok; ++j) {
-          const int tok = at.span.tile(at.u0 + j) * kPreTile;
-          ok = pre_wait(s_full + tile, s_phase & 1, &s_abort, 42);
+        for (int j = 0; j < n_groups && ok; ++j) {
+          const int tok = at.span.tile(at.u0 + (j >> 1)) * kPreTile + 64 * (j & 1);
+          const uint32_t buffer = s_phase & 1, t_b = t_s + 64 * buffer;
+          ok = pre_wait(s_full + 2 * tile + buffer, (s_phase >> 1) & 1, &s_abort, 42);
           tc_fence_after();
           if (j == 0) {  // (written before the queries were handed to the products that have just finished)
             mul = q_mul[(segments & 1) * kPreRows + tile * 128 + row_in];
@@ -245,47 +254,38 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             mul = finite ? mul : 1.0f;
             ++segments;
           }
-          const uint32_t got = valid[(seen + j) & 3];
-          const bool whole = got == 0x03030303u && tok + kPreTile <= kv && tok + kPreTile <= at.span.p_lo + 1 &&
-                             (a.m.window == 0 || tok > at.span.p_hi - a.m.window || tok + kPreTile <= a.m.sinks);
+          const uint32_t got = (valid[(seen + (j >> 1)) & 3] >> (16 * (j & 1))) & 0xFFFFu;
+          const bool whole = got == 0x0303u && tok + 64 <= kv && tok + 64 <= at.span.p_lo + 1 &&
+                             (a.m.window == 0 || tok > at.span.p_hi - a.m.window || tok + 64 <= a.m.sinks);
           auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u; };
-          // Scores are read twice, 64 at a time: first their maximum, and hidden ones go back as -inf.  (Held in registers, all 128
-          // take the code and the registers that keep the other warps from running: 1018 us against 806 for 8 prompts of 2048.)
           uint32_t s[64];
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 64) {
-            tmem_ld_x32(t_s + c, s);
-            tmem_ld_x32(t_s + c + 32, s + 32);
-            tmem_ld_wait();
-            if (!whole) {
+          tmem_ld_x32(t_b, s);
+          tmem_ld_x32(t_b + 32, s + 32);
+          tmem_ld_wait();
+          if (!whole) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int t0 = tok + c + 32 * h;
-                const uint32_t pieces = got >> (c / 4 + 8 * h);
-                const uint32_t see = below(hi - t0) & (~below(lo - t0) | below(first - t0)) &
-                                     ((pieces & 1u ? 0xFFFFu : 0u) | (pieces & 2u ? 0xFFFF0000u : 0u));
+            for (int h = 0; h < 2; ++h) {
+              const int t0 = tok + 32 * h;
+              const uint32_t pieces = got >> (8 * h);
+              const uint32_t see = below(hi - t0) & (~below(lo - t0) | below(first - t0)) &
+                                   ((pieces & 1u ? 0xFFFFu : 0u) | (pieces & 2u ? 0xFFFF0000u : 0u));
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!((see >> e) & 1u)) s[32 * h + e] = 0xFF800000u;
-                tmem_st_x32(t_s + c + 32 * h, s + 32 * h);
-              }
+              for (int e = 0; e < 32; ++e)
+                if (!((see >> e) & 1u)) s[32 * h + e] = 0xFF800000u;
             }
-#pragma unroll
-            for (int e = 0; e < 64; e += 8)
-#pragma unroll
-              for (int f = 0; f < 4; ++f) top[f] = max3(top[f], __uint_as_float(s[e + f]), __uint_as_float(s[e + f + 4]));
           }
-          if (!whole) tmem_st_wait();
-          tmem_ld_x32(t_s, s);
-          tmem_ld_x32(t_s + 32, s + 32);
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 64; e += 8)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) top[f] = max3(top[f], __uint_as_float(s[e + f]), __uint_as_float(s[e + f + 4]));
           const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
           if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
             const float to = fmaxf(m, high), by = pre_exp2(m - to);
             m = to;
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
-              ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the tile before is in O
+              ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the groups before are in O
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -299,43 +299,40 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             }
           }
           const float2 mul2 = make_float2(mul, mul), low = make_float2(-m, -m);
-          // 64 scores into 32 columns of weights, over scores that have been read.  Sixteen at a time; sums and stores are a
-          // batch behind, or they would wait for every exponential: 662 cycles for 64 scores of a warp by itself, 1097 with sums
-          // in the order of the scores.
-#pragma unroll 1
-          for (int c = 0; c < 64; c += 32) {
-            tmem_ld_wait();
-            float2 w[2][8];
-            uint32_t p[16];
+          // 64 scores into 32 columns of weights, over the scores.  Sixteen at a time; sums and stores are a batch behind, or they
+          // would wait for every exponential: 662 cycles for 64 scores of a warp by itself, 1097 with sums in the order of the
+          // scores.
+          float2 w[2][8];
+          uint32_t p[16];
 #pragma unroll
-            for (int b = 0; b < 5; ++b) {
-              if (b < 4) {
+          for (int b = 0; b < 5; ++b) {
+            if (b < 4) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const float2 x = __ffma2_rn(
-                      make_float2(__uint_as_float(s[16 * b + 2 * e]), __uint_as_float(s[16 * b + 2 * e + 1])), mul2, low);
-                  w[b & 1][e] = make_float2(pre_exp2(x.x), pre_exp2(x.y));
-                }
-              }
-              if (b == 2 && c == 0) tmem_ld_x32(t_s + 64, s);
-              if (b > 0) {
-                const float2(&v)[8] = w[(b - 1) & 1];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[8 * ((b - 1) & 1) + e] = pre_half2(v[e].x, v[e].y);
-                l2 = __fadd2_rn(l2, __fadd2_rn(__fadd2_rn(__fadd2_rn(v[0], v[1]), __fadd2_rn(v[2], v[3])),
-                                               __fadd2_rn(__fadd2_rn(v[4], v[5]), __fadd2_rn(v[6], v[7]))));
-                if (((b - 1) & 1) == 1) pre_tmem_st_x16(t_s + c + 8 * (b - 2), p);
+              for (int e = 0; e < 8; ++e) {
+                const float2 x = __ffma2_rn(
+                    make_float2(__uint_as_float(s[16 * b + 2 * e]), __uint_as_float(s[16 * b + 2 * e + 1])), mul2, low);
+                w[b & 1][e] = make_float2(pre_exp2(x.x), pre_exp2(x.y));
               }
             }
-            if (c == 0) tmem_ld_x32(t_s + 96, s + 32);
+            if (b > 0) {
+              const float2(&v)[8] = w[(b - 1) & 1];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) p[8 * ((b - 1) & 1) + e] = pre_half2(v[e].x, v[e].y);
+              l2 = __fadd2_rn(l2, __fadd2_rn(__fadd2_rn(__fadd2_rn(v[0], v[1]), __fadd2_rn(v[2], v[3])),
+                                             __fadd2_rn(__fadd2_rn(v[4], v[5]), __fadd2_rn(v[6], v[7]))));
+              if (((b - 1) & 1) == 1) pre_tmem_st_x16(t_b + 8 * (b - 2), p);
+            }
           }
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(p_full + tile);
+          mbar_arrive(p_full + 2 * tile + buffer);
           ++s_phase;
         }
         // output of the row
         const float l = l2.x + l2.y;
+        // (scores are two groups ahead, so the last ones only show that the values of the third last are in; a barrier tells a
+        // phase from the next one, not from the one after that)
+        if (n_groups > 1) ok = ok && pre_wait(o_done + tile, s_phase & 1, &s_abort, 44);
         ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 44);
         tc_fence_after();
         const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
@@ -398,7 +395,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         }
         tc_fence_before();  // (the next segment's products over O come behind this row's next arrival)
       }
-      seen += n_tiles;
+      seen += at.u1 - at.u0;
       const bool begins = at.u0 == 0 && at.u1 < at.span.count;
       if (begins && threadIdx.x == 0) {
         Kv4Join j;
@@ -533,68 +530,61 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   } else if (warp == 12) {
     // ------------------------------------------------------------------------------------------------ products
     if (elect_one()) {
-      constexpr uint32_t kIdescS = pre_idesc(128, 128, false), kIdescO = pre_idesc(128, HD, true);
-      uint32_t q_phase = 0, q1_phase = 0, p_phase0 = 0, p_phase1 = 0, n = 0;  // n: token tiles so far
-      auto scores = [&](int tile, uint32_t stage, bool last) {
-        const uint32_t qa = base + L::kOffQ + tile * L::kOperand, ka = base + L::kOffK + stage * L::kOperand;
+      constexpr uint32_t kIdescS = pre_idesc(128, 64, false), kIdescO = pre_idesc(128, HD, true);
+      uint32_t q_phase[2] = {0, 0}, s_count[2] = {0, 0}, o_count[2] = {0, 0}, n = 0;  // n: token tiles so far
+      auto scores = [&](int tile, uint32_t stage, int half, bool last) {
+        const uint32_t qa = base + L::kOffQ + tile * L::kOperand, ka = base + L::kOffK + stage * L::kOperand + half * 8192;
+        const uint32_t buffer = s_count[tile]++ & 1;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          pre_mma_ss(tmem + tile * 128, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
+          pre_mma_ss(tmem + tile * 128 + buffer * 64, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
                      umma_desc_k_sw128(ka + (k >> 2) * L::kHalf + (k & 3) * 32), kIdescS, k > 0);
-        umma_commit(s_full + tile);
+        umma_commit(s_full + 2 * tile + buffer);
         if (last) umma_commit(q_empty + tile);
       };
-      auto values = [&](int tile, uint32_t stage, bool add) {
-        const uint32_t va = base + L::kOffV + stage * L::kOperand;
+      auto values = [&](int tile, uint32_t stage, int half, bool add) {
+        const uint32_t va = base + L::kOffV + stage * L::kOperand + half * 8192;
+        const uint32_t buffer = o_count[tile] & 1;
+        ok = pre_wait(p_full + 2 * tile + buffer, (o_count[tile]++ >> 1) & 1, &s_abort, 51);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < kPreTile / 16; ++k)
-          pre_mma_ts(tmem + 256 + tile * HD, tmem + tile * 128 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf), kIdescO,
-                     add || k > 0);
+        for (int k = 0; k < 4; ++k)
+          pre_mma_ts(tmem + 256 + tile * HD, tmem + tile * 128 + buffer * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf),
+                     kIdescO, add || k > 0);
         umma_commit(o_done + tile);
       };
+      // Scores run two groups of 64 tokens ahead of values, so that the softmax warps find the next group's when they have
+      // handed over one.  A buffer's weights are read before the scores over them are computed: products run in order.
       for (;;) {
-        const int rows = at.seq.n * a.g.G - at.rt * kPreRows, n_tiles = at.u1 - at.u0;
-        const bool two = rows > 128;
-        ok = ok && pre_wait(q_full, q_phase & 1, &s_abort, 47);
-        ++q_phase;
-        if (two) {
-          ok = ok && pre_wait(q_full + 1, q1_phase & 1, &s_abort, 48);
-          ++q1_phase;
-        }
+        const int rows = at.seq.n * a.g.G - at.rt * kPreRows, groups = pre_groups(a.c, at);
+        const int tiles = rows > 128 ? 2 : 1;
+        for (int t = 0; t < tiles; ++t) ok = ok && pre_wait(q_full + t, q_phase[t]++ & 1, &s_abort, 47);
         ok = ok && pre_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
         if (!ok) break;
         tc_fence_after();
-        scores(0, n % kPreStages, n_tiles == 1);
-        if (two) scores(1, n % kPreStages, n_tiles == 1);
+#pragma unroll 1
+        for (int i = 0; i < 2 && i < groups; ++i)
+          for (int t = 0; t < tiles; ++t) scores(t, n % kPreStages, i, i + 1 == groups);
         umma_commit(k_empty + n % kPreStages);
-        for (int j = 0; j < n_tiles && ok; ++j, ++n) {
-          const uint32_t stage = n % kPreStages, next = (n + 1) % kPreStages;
-          const bool last = j + 1 == n_tiles;
-          ok = pre_wait(v_full + stage, (n / kPreStages) & 1, &s_abort, 50);
-          ok = ok && pre_wait(p_full, p_phase0 & 1, &s_abort, 51);
-          ++p_phase0;
-          tc_fence_after();
+#pragma unroll 1
+        for (int i = 0; i < groups && ok; ++i) {
+          const uint32_t at_v = n + (i >> 1), at_k = n + ((i + 2) >> 1), half = i & 1;
+          if (half == 0) ok = pre_wait(v_full + at_v % kPreStages, (at_v / kPreStages) & 1, &s_abort, 50);
+          const bool ahead = i + 2 < groups;
+          if (ahead && half == 0) ok = ok && pre_wait(k_full + at_k % kPreStages, (at_k / kPreStages) & 1, &s_abort, 52);
           if (!ok) break;
-          values(0, stage, j > 0);
-          if (!last) {
-            ok = pre_wait(k_full + next, ((n + 1) / kPreStages) & 1, &s_abort, 52);
-            if (!ok) break;
-            tc_fence_after();
-            scores(0, next, j + 2 == n_tiles);
+          tc_fence_after();
+#pragma unroll 1
+          for (int t = 0; t < tiles && ok; ++t) {
+            values(t, at_v % kPreStages, half, i > 0);
+            if (ahead && ok) scores(t, at_k % kPreStages, half, i + 3 == groups);
           }
-          if (two) {
-            ok = pre_wait(p_full + 1, p_phase1 & 1, &s_abort, 53);
-            ++p_phase1;
-            if (!ok) break;
-            tc_fence_after();
-            values(1, stage, j > 0);
-          }
-          umma_commit(v_empty + stage);
-          if (!last) {
-            if (two) scores(1, next, j + 2 == n_tiles);
-            umma_commit(k_empty + next);
-          }
+          if (!ok) break;
+          if (half == 1 || i + 1 == groups) umma_commit(v_empty + at_v % kPreStages);
+          if (ahead && (half == 1 || i + 3 == groups)) umma_commit(k_empty + at_k % kPreStages);
         }
+        n += at.u1 - at.u0;
         if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
       }
     }
