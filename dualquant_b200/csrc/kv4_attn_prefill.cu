@@ -32,7 +32,7 @@ struct PreSmem {
   static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
   static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
   static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
-  static constexpr int kBars = 4 + 4 * kPreStages + 10;
+  static constexpr int kBars = 4 + 4 * kPreStages + 12;
   static constexpr int kOffValid = kOffBar + kBars * 8;
   static constexpr int kOffMul = kOffValid + 4 * 4;            // [2][256] what a row's scores have to be multiplied with
   static constexpr int kOffCursor = kOffMul + 2 * kPreRows * 4;
@@ -165,7 +165,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   uint64_t* v_empty = v_full + kPreStages;
   uint64_t* s_full = v_empty + kPreStages;      // [row tile][buffer] scores are in tensor memory
   uint64_t* p_full = s_full + 4;                // [row tile][buffer] weights are
-  uint64_t* o_done = p_full + 4;                // [row tile] 64 tokens' values are in its output
+  uint64_t* o_done = p_full + 4;                // [row tile][buffer] the values of its weights are in the output
   float* q_mul = reinterpret_cast<float*>(smem + L::kOffMul);
   // pieces of 16 tokens that are there, of the last four tiles: two bits in each of four bytes (warps 8 to 11)
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kOffValid);
@@ -177,10 +177,10 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 32 * kPreLoaders);
       mbar_init(q_empty + i, 1);
-      mbar_init(o_done + i, 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
+      mbar_init(o_done + i, 1);
       mbar_init(p_full + i, 128);
     }
     for (int i = 0; i < kPreStages; ++i) {
@@ -285,7 +285,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             m = to;
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
-              ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 43);  // the groups before are in O
+              // the groups before are in O.  (A barrier of its own for each buffer: scores are two groups ahead, so they show that
+              // the third last group is in, and a barrier's phase cannot be told from the one two later.)
+              ok = ok && pre_wait(o_done + 2 * tile + ((s_phase - 1) & 1), ((s_phase - 1) >> 1) & 1, &s_abort, 43);
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -330,10 +332,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         }
         // output of the row
         const float l = l2.x + l2.y;
-        // (scores are two groups ahead, so the last ones only show that the values of the third last are in; a barrier tells a
-        // phase from the next one, not from the one after that)
-        if (n_groups > 1) ok = ok && pre_wait(o_done + tile, s_phase & 1, &s_abort, 44);
-        ok = ok && pre_wait(o_done + tile, (s_phase - 1) & 1, &s_abort, 44);
+        ok = ok && pre_wait(o_done + 2 * tile + ((s_phase - 1) & 1), ((s_phase - 1) >> 1) & 1, &s_abort, 44);
         tc_fence_after();
         const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
         // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
@@ -552,7 +551,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         for (int k = 0; k < 4; ++k)
           pre_mma_ts(tmem + 256 + tile * HD, tmem + tile * 128 + buffer * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf),
                      kIdescO, add || k > 0);
-        umma_commit(o_done + tile);
+        umma_commit(o_done + 2 * tile + buffer);
       };
       // Scores run two groups of 64 tokens ahead of values, so that the softmax warps find the next group's when they have
       // handed over one.  A buffer's weights are read before the scores over them are computed: products run in order.
