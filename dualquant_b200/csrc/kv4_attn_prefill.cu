@@ -6,7 +6,8 @@
 //                    weights back to tensor memory, at the end the output
 //   warps 8-11       codes from the pages to fp16 keys and values (fma(c, scale, zero), one rounding) in shared memory
 //   warp 12          issues the products: S = Q K' (both from shared memory), O += P V (P from tensor memory)
-//   warps 13-15      queries of the next segment into shared memory as soon as its predecessor's last scores are computed
+//   warps 13-15      queries of the next segment into shared memory as soon as its predecessor's last scores are computed; the
+//                    softmax warps make operands of them before they write their outputs
 // Softmax goes by groups of 64 tokens, whose scores a thread holds in registers.  Tensor memory (512 columns): two buffers of 64
 // scores for each row tile (weights take the first half of their scores' columns) and the outputs of both.
 //
@@ -32,10 +33,10 @@ struct PreSmem {
   static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
   static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
   static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
-  static constexpr int kBars = 4 + 4 * kPreStages + 12;
+  static constexpr int kBars = 6 + 4 * kPreStages + 12;
   static constexpr int kOffValid = kOffBar + kBars * 8;
-  static constexpr int kOffMul = kOffValid + 4 * 4;            // [2][256] what a row's scores have to be multiplied with
-  static constexpr int kOffCursor = kOffMul + 2 * kPreRows * 4;
+  static constexpr int kOffMul = kOffValid + 4 * 4;            // [256] what a row's scores have to be multiplied with
+  static constexpr int kOffCursor = kOffMul + kPreRows * 4;
   static constexpr int kOffTmem = kOffCursor + static_cast<int>((sizeof(Kv4Cursor) + 8 + 15) / 16 * 16);
   static constexpr int kBytes = kOffTmem + 16 + 1024;  // (the operands start at a multiple of 1024)
 };
@@ -157,9 +158,10 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
-  uint64_t* q_full = bar;                       // [2] a row tile's queries are in shared memory
+  uint64_t* q_full = bar;                       // [2] a row tile's queries are in shared memory, as operands
   uint64_t* q_empty = bar + 2;                  // [2] its last scores have been computed
-  uint64_t* k_full = bar + 4;                   // [stage]
+  uint64_t* q_raw = bar + 4;                    // [2] they are as they came
+  uint64_t* k_full = bar + 6;                   // [stage]
   uint64_t* k_empty = k_full + kPreStages;
   uint64_t* v_full = k_empty + kPreStages;
   uint64_t* v_empty = v_full + kPreStages;
@@ -175,7 +177,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 32 * kPreLoaders);
+      mbar_init(q_full + i, 128);
+      mbar_init(q_raw + i, 32 * kPreLoaders);
       mbar_init(q_empty + i, 1);
     }
     for (int i = 0; i < 4; ++i) {
@@ -224,36 +227,178 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
     uint32_t s_phase = 0;  // groups of 64 tokens so far
     int seen = 0;          // token tiles of the call, both row tiles'
-    uint32_t segments = 0;  // segments of this row tile
-    bool is_first = true, goes_on = false;
-    for (;; is_first = false) {
-      const int rows = at.seq.n * a.g.G - at.rt * kPreRows;  // of the segment, 256 at most count
-      const int n_groups = pre_groups(a.c, at);
-      const int r = at.rt * kPreRows + tile * 128 + row_in;
-      const bool there = tile * 128 + row_in < rows;
-      const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
-      const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
+    uint32_t q_uses = 0;
+    bool is_first = true, goes_on = false, fresh = true, more = true;
+    Kv4Cursor next = at;
+    float mul = 1.0f, m = kKv4NoMax;
+    float2 l2 = make_float2(0.0f, 0.0f);
+    bool finite = true;
+    // One round: the queries of the next segment, so that its scores are computed meanwhile; the output of this segment; the
+    // groups of the next.  (First round: no output.)
+    for (;;) {
+      float mul_next = 1.0f;
+      if (more && ok && (tile == 0 || next.seq.n * a.g.G - next.rt * kPreRows > 128)) {
+        // A row as fp16 times a power of two that brings its largest element to [2^14, 2^15): HD / 16 lanes a row, in place
+        constexpr int kRowLanes = HD / 16, kRowsAtOnce = 32 / kRowLanes;
+        const int l = lane % kRowLanes;
+        uint8_t* const dst = smem + L::kOffQ + tile * L::kOperand + (l >> 2) * L::kHalf;
+        auto place = [&](int row, int c) { return dst + row * 128 + (((((2 * l) & 7) + c) ^ (row & 7)) << 4); };
+        float* mul_out = q_mul + tile * 128;
+        ok = pre_wait(q_raw + tile, q_uses++ & 1, &s_abort, 56);
+#pragma unroll 1
+        for (int row = (warp & 3) * 32 + lane / kRowLanes; row < (warp & 3) * 32 + 32; row += kRowsAtOnce) {
+          const uint4 v[2] = {*reinterpret_cast<const uint4*>(place(row, 0)), *reinterpret_cast<const uint4*>(place(row, 1))};
+          uint32_t big = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            big = __vmaxu2(big, __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
+                                         __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
+          big = max(big & 0xFFFFu, big >> 16);
+          // Ordinary rows, largest element in [2^-10, 2^15), are fp16 as they are (what lies below 2^-14 of them is off by 2^-25
+          // at most); if one of the warp's rows is not, the factors of all of them are looked up.
+          const uint32_t small = __ballot_sync(0xFFFFFFFFu, big < 0x3A80u);
+          constexpr uint32_t kRowMask = (1u << kRowLanes) - 1u;
+          const bool odd = big >= 0x4700u || ((small >> (lane & ~(kRowLanes - 1))) & kRowMask) == kRowMask;
+          bool finite_row = true;
+          float by = 1.0f, mul_row = fmaxf(fabsf(a.scale2), 1.2e-38f);
+          if (__any_sync(0xFFFFFFFFu, odd)) {
+#pragma unroll
+            for (int d = 1; d < kRowLanes; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+            finite_row = big < 0x7F80u;  // no infinity and no NaN; rows that are not finite are made zero here
+            const int e = big > 0 && finite_row ? static_cast<int>(big >> 7) - 127 : 0;
+            const int up = max(min(14 - e, 100), -103);
+            by = __int_as_float((up + 127) << 23);
+            mul_row = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
+          }
+          if (a.scale2 < 0.0f) by = -by;  // (the maximum is taken of scores times |scale|)
+          if (a.scale2 == 0.0f) by = 0.0f, mul_row = 1.0f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {  // elements 2j, 2j + 1 and 2j + 4, 2j + 5
+              const uint32_t p = finite_row ? x[j] : 0u, q = finite_row ? x[j + 2] : 0u;
+              h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
+              h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
+            }
+            *reinterpret_cast<uint4*>(place(row, i)) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+          if (l == 0) mul_out[row] = finite_row ? mul_row : __int_as_float(0x7FC00000);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full + tile);
+        __syncwarp();
+        mul_next = mul_out[row_in];
+      }
+      if (!fresh) {
+        const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
+        if (tile == 0 || rows > 128) {
+          const int r = at.rt * kPreRows + tile * 128 + row_in;
+          const bool there = tile * 128 + row_in < rows;
+          const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
+          const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
+          // output of the row
+          const float l = l2.x + l2.y;
+          ok = ok && pre_wait(o_done + 2 * tile + ((s_phase - 1) & 1), ((s_phase - 1) >> 1) & 1, &s_abort, 44);
+          tc_fence_after();
+          const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
+          // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
+          float by = whole_segment ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
+          if (!finite && l != 0.0f) by = __int_as_float(0x7FC00000);
+          float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(kPreRows, HD);
+          float* part_o = part + 2 * kPreRows + (tile * 128 + row_in) * HD;
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tmem_ld_x32(t_o + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int g = 0; g < 32; g += 8) {  // elements into their own order
+              float v[8];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] = __uint_as_float(o[g + 2 * e]) * by;
+                v[e + 4] = __uint_as_float(o[g + 2 * e + 1]) * by;
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[g + e] = __float_as_uint(l == 0.0f ? 0.0f : v[e]);
+            }
+            if (whole_segment) {
+              // four lanes exchange their 64 bytes so that they store one row together, then the next
+              uint4 x[4];
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const float* v = reinterpret_cast<const float*>(o + 8 * g);
+                x[g] = make_uint4(pre_bf16x2(v[0], v[1]), pre_bf16x2(v[2], v[3]), pre_bf16x2(v[4], v[5]), pre_bf16x2(v[6], v[7]));
+              }
+#pragma unroll
+              for (int d = 1; d < 4; d <<= 1) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  if (g & d) continue;
+                  const bool up = lane & d;  // gives x[g], keeps x[g + d]
+                  const uint4 give = up ? x[g] : x[g + d];
+                  const uint4 take = make_uint4(__shfl_xor_sync(0xFFFFFFFFu, give.x, d), __shfl_xor_sync(0xFFFFFFFFu, give.y, d),
+                                                __shfl_xor_sync(0xFFFFFFFFu, give.z, d), __shfl_xor_sync(0xFFFFFFFFu, give.w, d));
+                  if (up) x[g] = take;
+                  else x[g + d] = take;
+                }
+              }
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {  // 16 bytes lane % 4 of the row of lane (lane & ~3) + g
+                const long long row_at = __shfl_sync(0xFFFFFFFFu, there ? static_cast<long long>(out_at) : -1ll, (lane & ~3) + g);
+                if (row_at >= 0 && ok) *reinterpret_cast<uint4*>(a.out + row_at + c + 8 * (lane & 3)) = x[g];
+              }
+            } else if (there && ok) {
+#pragma unroll
+              for (int g = 0; g < 32; g += 4)
+                *reinterpret_cast<uint4*>(part_o + c + g) = make_uint4(o[g], o[g + 1], o[g + 2], o[g + 3]);
+            }
+          }
+          if (!whole_segment && there) {
+            part[2 * (tile * 128 + row_in)] = m;
+            part[2 * (tile * 128 + row_in) + 1] = l;
+          }
+          tc_fence_before();  // (the next segment's products over O come behind this row's next arrival)
+        }
+        seen += at.u1 - at.u0;
+        const bool begins = at.u0 == 0 && at.u1 < at.span.count;
+        if (begins && threadIdx.x == 0) {
+          Kv4Join j;
+          j.parts = 1 + (at.span.count - at.u1 + share - 1) / share;
+          j.slot = is_first ? 0 : 1;
+          j.rows = min(rows, kPreRows);
+          j.first_row = at.rt * kPreRows;
+          j.row0 = at.seq.row0;
+          j.h = at.h;
+          a.join[blockIdx.x] = j;
+        }
+        goes_on |= begins;
+        is_first = false;
+      }
+      if (!more || !ok) break;
+      at = next;
+      fresh = false;
+      const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
       if (tile == 0 || rows > 128) {
+        const int n_groups = pre_groups(a.c, at);
+        const bool there = tile * 128 + row_in < rows;
+        const int i_tok = there ? a.g.by(at.rt * kPreRows + tile * 128 + row_in) : 0;
         const int kv = min(at.seq.kv, a.c.capacity);
         const int p_row = at.seq.kv - at.seq.n + i_tok;
         const int hi = there ? min(p_row + 1, kv) : 0;                   // tokens lo ... hi - 1 and those below `first`
         const int lo = a.m.window > 0 ? p_row - a.m.window + 1 : 0;
         const int first = a.m.window > 0 ? min(a.m.sinks, hi) : 0;
-        float m = kKv4NoMax;
-        float2 l2 = make_float2(0.0f, 0.0f);
-        float mul = 0.0f;
-        bool finite = true;
+        m = kKv4NoMax;
+        l2 = make_float2(0.0f, 0.0f);
+        finite = !isnan(mul_next);
+        mul = finite ? mul_next : 1.0f;
         for (int j = 0; j < n_groups && ok; ++j) {
           const int tok = at.span.tile(at.u0 + (j >> 1)) * kPreTile + 64 * (j & 1);
           const uint32_t buffer = s_phase & 1, t_b = t_s + 64 * buffer;
           ok = pre_wait(s_full + 2 * tile + buffer, (s_phase >> 1) & 1, &s_abort, 42);
           tc_fence_after();
-          if (j == 0) {  // (written before the queries were handed to the products that have just finished)
-            mul = q_mul[(segments & 1) * kPreRows + tile * 128 + row_in];
-            finite = !isnan(mul);
-            mul = finite ? mul : 1.0f;
-            ++segments;
-          }
           const uint32_t got = (valid[(seen + (j >> 1)) & 3] >> (16 * (j & 1))) & 0xFFFFu;
           const bool whole = got == 0x0303u && tok + 64 <= kv && tok + 64 <= at.span.p_lo + 1 &&
                              (a.m.window == 0 || tok > at.span.p_hi - a.m.window || tok + 64 <= a.m.sinks);
@@ -330,84 +475,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           mbar_arrive(p_full + 2 * tile + buffer);
           ++s_phase;
         }
-        // output of the row
-        const float l = l2.x + l2.y;
-        ok = ok && pre_wait(o_done + 2 * tile + ((s_phase - 1) & 1), ((s_phase - 1) >> 1) & 1, &s_abort, 44);
-        tc_fence_after();
-        const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
-        // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
-        float by = whole_segment ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
-        if (!finite && l != 0.0f) by = __int_as_float(0x7FC00000);
-        float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(kPreRows, HD);
-        float* part_o = part + 2 * kPreRows + (tile * 128 + row_in) * HD;
-#pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t o[32];
-          tmem_ld_x32(t_o + c, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int g = 0; g < 32; g += 8) {  // elements into their own order
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[e] = __uint_as_float(o[g + 2 * e]) * by;
-              v[e + 4] = __uint_as_float(o[g + 2 * e + 1]) * by;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[g + e] = __float_as_uint(l == 0.0f ? 0.0f : v[e]);
-          }
-          if (whole_segment) {
-            // four lanes exchange their 64 bytes so that they store one row together, then the next
-            uint4 x[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float* v = reinterpret_cast<const float*>(o + 8 * g);
-              x[g] = make_uint4(pre_bf16x2(v[0], v[1]), pre_bf16x2(v[2], v[3]), pre_bf16x2(v[4], v[5]), pre_bf16x2(v[6], v[7]));
-            }
-#pragma unroll
-            for (int d = 1; d < 4; d <<= 1) {
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                if (g & d) continue;
-                const bool up = lane & d;  // gives x[g], keeps x[g + d]
-                const uint4 give = up ? x[g] : x[g + d];
-                const uint4 take = make_uint4(__shfl_xor_sync(0xFFFFFFFFu, give.x, d), __shfl_xor_sync(0xFFFFFFFFu, give.y, d),
-                                              __shfl_xor_sync(0xFFFFFFFFu, give.z, d), __shfl_xor_sync(0xFFFFFFFFu, give.w, d));
-                if (up) x[g] = take;
-                else x[g + d] = take;
-              }
-            }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {  // 16 bytes lane % 4 of the row of lane (lane & ~3) + g
-              const long long row_at = __shfl_sync(0xFFFFFFFFu, there ? static_cast<long long>(out_at) : -1ll, (lane & ~3) + g);
-              if (row_at >= 0 && ok) *reinterpret_cast<uint4*>(a.out + row_at + c + 8 * (lane & 3)) = x[g];
-            }
-          } else if (there && ok) {
-#pragma unroll
-            for (int g = 0; g < 32; g += 4)
-              *reinterpret_cast<uint4*>(part_o + c + g) = make_uint4(o[g], o[g + 1], o[g + 2], o[g + 3]);
-          }
-        }
-        if (!whole_segment && there) {
-          part[2 * (tile * 128 + row_in)] = m;
-          part[2 * (tile * 128 + row_in) + 1] = l;
-        }
-        tc_fence_before();  // (the next segment's products over O come behind this row's next arrival)
       }
-      seen += at.u1 - at.u0;
-      const bool begins = at.u0 == 0 && at.u1 < at.span.count;
-      if (begins && threadIdx.x == 0) {
-        Kv4Join j;
-        j.parts = 1 + (at.span.count - at.u1 + share - 1) / share;
-        j.slot = is_first ? 0 : 1;
-        j.rows = min(rows, kPreRows);
-        j.first_row = at.rt * kPreRows;
-        j.row0 = at.seq.row0;
-        j.h = at.h;
-        a.join[blockIdx.x] = j;
-      }
-      goes_on |= begins;
-      if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
+      more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, next);
     }
     if (threadIdx.x == 0 && !goes_on) a.join[blockIdx.x].parts = 0;
   } else if (warp < 12) {
@@ -558,13 +627,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       for (;;) {
         const int rows = at.seq.n * a.g.G - at.rt * kPreRows, groups = pre_groups(a.c, at);
         const int tiles = rows > 128 ? 2 : 1;
-        for (int t = 0; t < tiles; ++t) ok = ok && pre_wait(q_full + t, q_phase[t]++ & 1, &s_abort, 47);
         ok = ok && pre_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
         if (!ok) break;
-        tc_fence_after();
 #pragma unroll 1
-        for (int i = 0; i < 2 && i < groups; ++i)
-          for (int t = 0; t < tiles; ++t) scores(t, n % kPreStages, i, i + 1 == groups);
+        for (int t = 0; t < tiles && ok; ++t) {
+          ok = pre_wait(q_full + t, q_phase[t]++ & 1, &s_abort, 47);
+          if (!ok) break;
+          tc_fence_after();
+          for (int i = 0; i < 2 && i < groups; ++i) scores(t, n % kPreStages, i, i + 1 == groups);
+        }
+        if (!ok) break;
         umma_commit(k_empty + n % kPreStages);
 #pragma unroll 1
         for (int i = 0; i < groups && ok; ++i) {
@@ -590,8 +662,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     __syncwarp();
   } else {
     // ------------------------------------------------------------------------------------------------ queries
-    // A row as fp16 times a power of two that brings its largest element to [2^14, 2^15), HD / 8 lanes a row.
-    // The rows come in by asynchronous copies, all of a row tile at once, and every lane converts the 16 bytes that it copied.
+    // All rows of a tile at once; the softmax warps make operands of them.
     constexpr int kRowLanes = HD / 16, kRowsAtOnce = 32 / kRowLanes, kStep = kPreLoaders * kRowsAtOnce;
     const int w = warp - 13, l = lane % kRowLanes, row0 = w * kRowsAtOnce + lane / kRowLanes;
     uint32_t uses[2] = {0, 0};
@@ -615,53 +686,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           pre_cp_async_16(smem_u32(place(row, 1)), src + 8, there ? 16 : 0);
         }
         asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
-        float* mul_out = q_mul + (use & 1) * kPreRows + tile * 128;
-#pragma unroll 1
-        for (int base_row = w * kRowsAtOnce; base_row < 128; base_row += kStep) {
-          const int row = base_row + lane / kRowLanes;
-          const bool in = row < 128;  // (the last round of HD 128 has rows for some of the warp's lanes only)
-          uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-          if (in) v[0] = *reinterpret_cast<const uint4*>(place(row, 0)), v[1] = *reinterpret_cast<const uint4*>(place(row, 1));
-          uint32_t big = 0;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            big = __vmaxu2(big, __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
-                                         __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
-          big = max(big & 0xFFFFu, big >> 16);
-          // Ordinary rows, largest element in [2^-10, 2^15), are fp16 as they are (what lies below 2^-14 of them is off by 2^-25
-          // at most); if one of the warp's rows is not, the factors of all of them are looked up.
-          const uint32_t small = __ballot_sync(0xFFFFFFFFu, big < 0x3A80u);
-          constexpr uint32_t kRowMask = (1u << kRowLanes) - 1u;
-          const bool odd = big >= 0x4700u || ((small >> (lane & ~(kRowLanes - 1))) & kRowMask) == kRowMask;
-          bool finite = true;
-          float by = 1.0f, mul = fmaxf(fabsf(a.scale2), 1.2e-38f);
-          if (__any_sync(0xFFFFFFFFu, odd)) {
-#pragma unroll
-            for (int d = 1; d < kRowLanes; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
-            finite = big < 0x7F80u;  // no infinity and no NaN; rows that are not finite are made zero here
-            const int e = big > 0 && finite ? static_cast<int>(big >> 7) - 127 : 0;
-            const int up = max(min(14 - e, 100), -103);
-            by = __int_as_float((up + 127) << 23);
-            mul = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
-          }
-          if (a.scale2 < 0.0f) by = -by;  // (the maximum is taken of scores times |scale|)
-          if (a.scale2 == 0.0f) by = 0.0f, mul = 1.0f;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            uint32_t h[4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {  // elements 2j, 2j + 1 and 2j + 4, 2j + 5
-              const uint32_t p = finite ? x[j] : 0u, q = finite ? x[j + 2] : 0u;
-              h[2 * j] = pre_half2(__uint_as_float(p << 16) * by, __uint_as_float(q << 16) * by);
-              h[2 * j + 1] = pre_half2(__uint_as_float(p & 0xFFFF0000u) * by, __uint_as_float(q & 0xFFFF0000u) * by);
-            }
-            if (in) *reinterpret_cast<uint4*>(place(row, i)) = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-          if (in && l == 0) mul_out[row] = finite ? mul : __int_as_float(0x7FC00000);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(q_full + tile);
+        mbar_arrive(q_raw + tile);
       }
       if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
     }
