@@ -394,14 +394,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         l2 = make_float2(0.0f, 0.0f);
         finite = !isnan(mul_next);
         mul = finite ? mul_next : 1.0f;
+        // groups from these tokens on are seen whole by every row
+        const int whole_hi = min(kv, at.span.p_lo + 1) - 64, whole_lo = a.m.window > 0 ? at.span.p_hi - a.m.window : -1,
+                  whole_sinks = a.m.window > 0 ? a.m.sinks - 64 : -1;
         for (int j = 0; j < n_groups && ok; ++j) {
           const int tok = at.span.tile(at.u0 + (j >> 1)) * kPreTile + 64 * (j & 1);
           const uint32_t buffer = s_phase & 1, t_b = t_s + 64 * buffer;
           ok = pre_wait(s_full + 2 * tile + buffer, (s_phase >> 1) & 1, &s_abort, 42);
           tc_fence_after();
           const uint32_t got = (valid[(seen + (j >> 1)) & 3] >> (16 * (j & 1))) & 0xFFFFu;
-          const bool whole = got == 0x0303u && tok + 64 <= kv && tok + 64 <= at.span.p_lo + 1 &&
-                             (a.m.window == 0 || tok > at.span.p_hi - a.m.window || tok + 64 <= a.m.sinks);
+          const bool whole = got == 0x0303u && tok <= whole_hi && (tok > whole_lo || tok <= whole_sinks);
           auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u; };
           uint32_t s[64];
           tmem_ld_x32(t_b, s);
@@ -545,6 +547,13 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // The lane's place in an operand: token w * 32 + in, its four 16-byte columns.  Lanes of the second 64 elements take their
+    // words in the order 2 3 0 1: the eight lanes that store together hit eight different columns.
+    const int turned = q & 2;
+    const uint32_t to_lane = (q >> 1) * L::kHalf + (w * 32 + in) * 128;
+    uint32_t column[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) column[e] = ((((q & 1) << 2) + (e ^ turned)) ^ (in & 7)) << 4;
     // keys of tile 0, values of tile 0, keys of tile 1 ...: one is converted while the next two are on the way
     look_up();
     seek();
@@ -561,25 +570,24 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
       if (!values && lane == 0)
         reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(got_now);
-      const uint8_t* from = raw + (values ? L::kRaw : 0);
-      // lanes of the second 64 elements take their words in the order 2 3 0 1: the eight lanes that store together hit eight
-      // different 16-byte columns
-      const int turned = q & 2;
-      uint8_t* to = smem + (values ? L::kOffV : L::kOffK) + stage * L::kOperand + (q >> 1) * L::kHalf;
-#pragma unroll 2
+      uint8_t* const from = raw + (values ? L::kRaw : 0);
+      // tokens that are not there become zeros: their weights are zero, and zero times what a slot may hold is not
+      if (left_now < 32 || got_now != 3u) {
+        if (lane >= left_now || !((got_now >> (lane >> 4)) & 1u)) reinterpret_cast<uint32_t*>(from + 32 * (HD / 2))[lane] = 0;
+        __syncwarp();
+      }
+      const uint8_t *src = from + in * (HD / 2) + q * 16, *pairs = from + 32 * (HD / 2) + in * 4;
+      uint8_t* const to = smem + (values ? L::kOffV : L::kOffK) + stage * L::kOperand + to_lane;
+#pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int t = i * kStep + in;
-        const uint8_t* src = from + t * (HD / 2) + q * 16;
-        const uint2 c01 = *reinterpret_cast<const uint2*>(src + 4 * turned), c23 = *reinterpret_cast<const uint2*>(src + (8 - 4 * turned));
-        __half2 pair = *reinterpret_cast<const __half2*>(from + 32 * (HD / 2) + t * 4);
-        // tokens that are not there become zeros: their weights are zero, and zero times what a slot may hold is not
-        if (t >= left_now || !((got_now >> (t >> 4)) & 1u)) pair = __half2half2(__ushort_as_half(0));
+        const uint2 c01 = *reinterpret_cast<const uint2*>(src + i * kStep * (HD / 2) + 4 * turned);
+        const uint2 c23 = *reinterpret_cast<const uint2*>(src + i * kStep * (HD / 2) + (8 - 4 * turned));
+        const __half2 pair = *reinterpret_cast<const __half2*>(pairs + i * kStep * 4);
         const __half2 sc = __low2half2(pair), ze = __high2half2(pair);
         const uint32_t c[4] = {c01.x, c01.y, c23.x, c23.y};
-        uint8_t* row = to + (w * 32 + t) * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint4*>(row + (((((q & 1) << 2) + (e ^ turned)) ^ (t & 7)) << 4)) = pre_expand(c[e], sc, ze);
+          *reinterpret_cast<uint4*>(to + column[e] + i * kStep * 128) = pre_expand(c[e], sc, ze);
       }
       fence_proxy_async_smem();
       mbar_arrive((values ? v_full : k_full) + stage);
