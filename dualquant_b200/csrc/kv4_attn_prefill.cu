@@ -8,8 +8,9 @@
 //   warp 12          issues the products: S = Q K' (both from shared memory), O += P V (P from tensor memory)
 //   warps 13-15      queries of the next segment into shared memory as soon as its predecessor's last scores are computed; the
 //                    softmax warps make operands of them before they write their outputs
-// Softmax goes by groups of 64 tokens, whose scores a thread holds in registers.  Tensor memory (512 columns): two buffers of 64
-// scores for each row tile (weights take the first half of their scores' columns) and the outputs of both.
+// Softmax goes by halves of a token tile, whose 64 scores a thread holds in registers; their weights are multiplied while the
+// other half's are taken.  Tensor memory (512 columns): 128 scores for each row tile (the weights of a half take the first half
+// of its scores' columns) and the outputs of both.
 //
 // Operands are fp16: a key or value of the cache is c * scale + zero with fp16 scale and zero, and 11 bits keep that to 2^-11
 // where bf16 would give 2^-8; queries (bf16) are exact in fp16 times a power of two of their row; weights lie in [0, 2^8].
@@ -33,7 +34,7 @@ struct PreSmem {
   static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
   static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
   static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
-  static constexpr int kBars = 6 + 4 * kPreStages + 12;
+  static constexpr int kBars = 6 + 4 * kPreStages + 10;
   static constexpr int kOffValid = kOffBar + kBars * 8;
   static constexpr int kOffMul = kOffValid + 4 * 4;            // [256] what a row's scores have to be multiplied with
   static constexpr int kOffCursor = kOffMul + kPreRows * 4;
@@ -165,9 +166,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   uint64_t* k_empty = k_full + kPreStages;
   uint64_t* v_full = k_empty + kPreStages;
   uint64_t* v_empty = v_full + kPreStages;
-  uint64_t* s_full = v_empty + kPreStages;      // [row tile][buffer] scores are in tensor memory
-  uint64_t* p_full = s_full + 4;                // [row tile][buffer] weights are
-  uint64_t* o_done = p_full + 4;                // [row tile][buffer] the values of its weights are in the output
+  uint64_t* s_full = v_empty + kPreStages;      // [row tile] scores of a token tile are in tensor memory
+  uint64_t* p_full = s_full + 2;                // [row tile][half] weights of 64 tokens are
+  uint64_t* o_done = p_full + 4;                // [row tile][half] the values of its weights are in the output
   float* q_mul = reinterpret_cast<float*>(smem + L::kOffMul);
   // pieces of 16 tokens that are there, of the last four tiles: two bits in each of four bytes (warps 8 to 11)
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kOffValid);
@@ -180,9 +181,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       mbar_init(q_full + i, 128);
       mbar_init(q_raw + i, 32 * kPreLoaders);
       mbar_init(q_empty + i, 1);
+      mbar_init(s_full + i, 1);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(s_full + i, 1);
       mbar_init(o_done + i, 1);
       mbar_init(p_full + i, 128);
     }
@@ -225,7 +226,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const int tile = warp >> 2, row_in = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes, in the upper half of an address
     const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
-    uint32_t s_phase = 0;  // groups of 64 tokens so far
+    uint32_t count[2] = {0, 0};  // first and second halves of token tiles so far
     int seen = 0;          // token tiles of the call, both row tiles'
     uint32_t q_uses = 0;
     bool is_first = true, goes_on = false, fresh = true, more = true;
@@ -300,7 +301,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
           // output of the row
           const float l = l2.x + l2.y;
-          ok = ok && pre_wait(o_done + 2 * tile + ((s_phase - 1) & 1), ((s_phase - 1) >> 1) & 1, &s_abort, 44);
+          const int last_half = (pre_groups(a.c, at) - 1) & 1;
+          ok = ok && pre_wait(o_done + 2 * tile + last_half, ((last_half ? count[1] : count[0]) - 1) & 1, &s_abort, 44);
           tc_fence_after();
           const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
           // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
@@ -399,9 +401,14 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
                   whole_sinks = a.m.window > 0 ? a.m.sinks - 64 : -1;
         for (int j = 0; j < n_groups && ok; ++j) {
           const int tok = at.span.tile(at.u0 + (j >> 1)) * kPreTile + 64 * (j & 1);
-          const uint32_t buffer = s_phase & 1, t_b = t_s + 64 * buffer;
-          ok = pre_wait(s_full + 2 * tile + buffer, (s_phase >> 1) & 1, &s_abort, 42);
-          tc_fence_after();
+          const int half = j & 1;
+          const uint32_t t_b = t_s + 64 * half;
+          if (half == 0) {
+            ok = pre_wait(s_full + tile, count[0]++ & 1, &s_abort, 42);
+            tc_fence_after();
+          } else {
+            ++count[1];
+          }
           const uint32_t got = (valid[(seen + (j >> 1)) & 3] >> (16 * (j & 1))) & 0xFFFFu;
           const bool whole = got == 0x0303u && tok <= whole_hi && (tok > whole_lo || tok <= whole_sinks);
           auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u; };
@@ -432,9 +439,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             m = to;
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
-              // the groups before are in O.  (A barrier of its own for each buffer: scores are two groups ahead, so they show that
-              // the third last group is in, and a barrier's phase cannot be told from the one two later.)
-              ok = ok && pre_wait(o_done + 2 * tile + ((s_phase - 1) & 1), ((s_phase - 1) >> 1) & 1, &s_abort, 43);
+              // the groups before are in O: those of earlier tiles are since there are scores of this one
+              if (half == 1) ok = ok && pre_wait(o_done + 2 * tile, (count[0] - 1) & 1, &s_abort, 43);
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -474,8 +480,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           }
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(p_full + 2 * tile + buffer);
-          ++s_phase;
+          mbar_arrive(p_full + 2 * tile + half);
         }
       }
       more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, next);
@@ -606,64 +611,66 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   } else if (warp == 12) {
     // ------------------------------------------------------------------------------------------------ products
     if (elect_one()) {
-      constexpr uint32_t kIdescS = pre_idesc(128, 64, false), kIdescO = pre_idesc(128, HD, true);
-      uint32_t q_phase[2] = {0, 0}, s_count[2] = {0, 0}, o_count[2] = {0, 0}, n = 0;  // n: token tiles so far
-      auto scores = [&](int tile, uint32_t stage, int half, bool last) {
-        const uint32_t qa = base + L::kOffQ + tile * L::kOperand, ka = base + L::kOffK + stage * L::kOperand + half * 8192;
-        const uint32_t buffer = s_count[tile]++ & 1;
+      constexpr uint32_t kIdescS = pre_idesc(128, 128, false), kIdescO = pre_idesc(128, HD, true);
+      uint32_t q_phase[2] = {0, 0}, p_phase[2][2] = {{0, 0}, {0, 0}}, n = 0;  // n: token tiles so far
+      auto scores = [&](int t, uint32_t tile_number, bool last) {
+        const uint32_t qa = base + L::kOffQ + t * L::kOperand, ka = base + L::kOffK + tile_number % kPreStages * L::kOperand;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          pre_mma_ss(tmem + tile * 128 + buffer * 64, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
+          pre_mma_ss(tmem + t * 128, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
                      umma_desc_k_sw128(ka + (k >> 2) * L::kHalf + (k & 3) * 32), kIdescS, k > 0);
-        umma_commit(s_full + 2 * tile + buffer);
-        if (last) umma_commit(q_empty + tile);
+        umma_commit(s_full + t);
+        if (last) umma_commit(q_empty + t);
       };
-      auto values = [&](int tile, uint32_t stage, int half, bool add) {
-        const uint32_t va = base + L::kOffV + stage * L::kOperand + half * 8192;
-        const uint32_t buffer = o_count[tile] & 1;
-        ok = pre_wait(p_full + 2 * tile + buffer, (o_count[tile]++ >> 1) & 1, &s_abort, 51);
+      auto values = [&](int t, uint32_t tile_number, int half, bool add) {
+        const uint32_t va = base + L::kOffV + tile_number % kPreStages * L::kOperand + half * 8192;
+        ok = ok && pre_wait(p_full + 2 * t + half, p_phase[t][half]++ & 1, &s_abort, 51);
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          pre_mma_ts(tmem + 256 + tile * HD, tmem + tile * 128 + buffer * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf),
-                     kIdescO, add || k > 0);
-        umma_commit(o_done + 2 * tile + buffer);
+          pre_mma_ts(tmem + 256 + t * HD, tmem + t * 128 + half * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf), kIdescO,
+                     add || k > 0);
+        umma_commit(o_done + 2 * t + half);
       };
-      // Scores run two groups of 64 tokens ahead of values, so that the softmax warps find the next group's when they have
-      // handed over one.  A buffer's weights are read before the scores over them are computed: products run in order.
+      // A row tile's next scores follow its weights' second half: products run in order, so those weights have been read.
       for (;;) {
-        const int rows = at.seq.n * a.g.G - at.rt * kPreRows, groups = pre_groups(a.c, at);
-        const int tiles = rows > 128 ? 2 : 1;
+        const int rows = at.seq.n * a.g.G - at.rt * kPreRows, groups = pre_groups(a.c, at), tiles = (groups + 1) / 2;
+        const bool two = rows > 128;
         ok = ok && pre_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
+        ok = ok && pre_wait(q_full, q_phase[0]++ & 1, &s_abort, 47);
         if (!ok) break;
-#pragma unroll 1
-        for (int t = 0; t < tiles && ok; ++t) {
-          ok = pre_wait(q_full + t, q_phase[t]++ & 1, &s_abort, 47);
+        tc_fence_after();
+        scores(0, n, tiles == 1);
+        if (two) {
+          ok = pre_wait(q_full + 1, q_phase[1]++ & 1, &s_abort, 48);
           if (!ok) break;
           tc_fence_after();
-          for (int i = 0; i < 2 && i < groups; ++i) scores(t, n % kPreStages, i, i + 1 == groups);
+          scores(1, n, tiles == 1);
         }
-        if (!ok) break;
         umma_commit(k_empty + n % kPreStages);
 #pragma unroll 1
-        for (int i = 0; i < groups && ok; ++i) {
-          const uint32_t at_v = n + (i >> 1), at_k = n + ((i + 2) >> 1), half = i & 1;
-          if (half == 0) ok = pre_wait(v_full + at_v % kPreStages, (at_v / kPreStages) & 1, &s_abort, 50);
-          const bool ahead = i + 2 < groups;
-          if (ahead && half == 0) ok = ok && pre_wait(k_full + at_k % kPreStages, (at_k / kPreStages) & 1, &s_abort, 52);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int t = 0; t < tiles && ok; ++t) {
-            values(t, at_v % kPreStages, half, i > 0);
-            if (ahead && ok) scores(t, at_k % kPreStages, half, i + 3 == groups);
+        for (int j = 0; j < tiles && ok; ++j, ++n) {
+          const bool more = j + 1 < tiles, both = 2 * j + 1 < groups;
+          ok = pre_wait(v_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 50);
+          values(0, n, 0, j > 0);
+          if (both) values(0, n, 1, true);
+          if (more) {
+            ok = ok && pre_wait(k_full + (n + 1) % kPreStages, ((n + 1) / kPreStages) & 1, &s_abort, 52);
+            if (!ok) break;
+            tc_fence_after();
+            scores(0, n + 1, j + 2 == tiles);
+          }
+          if (two) {
+            values(1, n, 0, j > 0);
+            if (both) values(1, n, 1, true);
+            if (!ok) break;
+            if (more) scores(1, n + 1, j + 2 == tiles);
           }
           if (!ok) break;
-          if (half == 1 || i + 1 == groups) umma_commit(v_empty + at_v % kPreStages);
-          if (ahead && (half == 1 || i + 3 == groups)) umma_commit(k_empty + at_k % kPreStages);
+          umma_commit(v_empty + n % kPreStages);
+          if (more) umma_commit(k_empty + (n + 1) % kPreStages);
         }
-        n += at.u1 - at.u0;
         if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
       }
     }
