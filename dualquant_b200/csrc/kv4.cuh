@@ -61,15 +61,27 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Batch& c, int b) {
   return s;
 }
 
-// Sequence of a token row (c.B: none), found by a whole warp: one round of loads for every 32 sequences.
-__device__ __forceinline__ int kv4_seq_of_row(const Kv4Batch& c, int row, int lane) {
-  if (c.cu_new == nullptr) return row / (c.T / c.B);
-  int b = 0;
-  for (int base = 0; base < c.B; base += 32) {
-    const bool before = base + lane < c.B && c.cu_new[base + lane + 1] <= row;
-    b += __popc(__ballot_sync(0xFFFFFFFFu, before));
+// Sequence and position of a token row (c.B: it belongs to none), found by a whole warp with one round of loads for every 32
+// sequences.
+__device__ __forceinline__ int kv4_find(const Kv4Batch& c, int row, int lane, int* pos) {
+  if (c.cu_new == nullptr) {
+    const int n = c.T / c.B, b = row / n;
+    *pos = min(max(c.kv_len[b], 0), kKv4Far) - n + (row - b * n);
+    return b;
   }
-  return b;
+  for (int base = 0; base < c.B; base += 32) {
+    const int b = base + lane;
+    Kv4Seq s = {0, 0, 0};
+    if (b < c.B) s = kv4_seq(c, b);
+    const uint32_t mine = __ballot_sync(0xFFFFFFFFu, row >= s.row0 && row - s.row0 < s.n);
+    if (mine != 0) {
+      const int l = __ffs(mine) - 1;
+      *pos = __shfl_sync(0xFFFFFFFFu, s.kv - s.n + (row - s.row0), l);
+      return base + l;
+    }
+  }
+  *pos = -1;
+  return c.B;
 }
 
 // ------------------------------------------------------------------------------------------------------------------

@@ -100,30 +100,6 @@ __device__ __forceinline__ uint32_t pre_bf16x2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// mbar_wait with a hint of how long the wait may sleep: sixteen warps share the issue slots, most of them waiting.
-__device__ __forceinline__ bool pre_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int site) {
-  auto ready = [&]() {
-    uint32_t done;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\nselp.b32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-  };
-  if (ready()) return true;
-  const long long t0 = clock64();
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i)
-      if (ready()) return true;
-    if (*abort_flag != 0) return false;
-    if (clock64() - t0 > (1ll << 31)) {
-      *abort_flag = site;
-      return false;
-    }
-  }
-}
 // eight codes -> fp16 c * scale + zero, elements 0 4 1 5 2 6 3 7
 __device__ __forceinline__ uint4 pre_expand(uint32_t w, __half2 s, __half2 z) {
   const __half2 k1024 = __half2half2(__ushort_as_half(0x6400)), k16th = __half2half2(__ushort_as_half(0x2C00)),
@@ -245,7 +221,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         uint8_t* const dst = smem + L::kOffQ + tile * L::kOperand + (l >> 2) * L::kHalf;
         auto place = [&](int row, int c) { return dst + row * 128 + (((((2 * l) & 7) + c) ^ (row & 7)) << 4); };
         float* mul_out = q_mul + tile * 128;
-        ok = pre_wait(q_raw + tile, q_uses++ & 1, &s_abort, 56);
+        ok = mbar_wait(q_raw + tile, q_uses++ & 1, &s_abort, 56);
 #pragma unroll 1
         for (int row = (warp & 3) * 32 + lane / kRowLanes; row < (warp & 3) * 32 + 32; row += kRowsAtOnce) {
           const uint4 v[2] = {*reinterpret_cast<const uint4*>(place(row, 0)), *reinterpret_cast<const uint4*>(place(row, 1))};
@@ -302,7 +278,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           // output of the row
           const float l = l2.x + l2.y;
           const int last_half = (pre_groups(a.c, at) - 1) & 1;
-          ok = ok && pre_wait(o_done + 2 * tile + last_half, ((last_half ? count[1] : count[0]) - 1) & 1, &s_abort, 44);
+          ok = ok && mbar_wait(o_done + 2 * tile + last_half, ((last_half ? count[1] : count[0]) - 1) & 1, &s_abort, 44);
           tc_fence_after();
           const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
           // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
@@ -404,7 +380,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           const int half = j & 1;
           const uint32_t t_b = t_s + 64 * half;
           if (half == 0) {
-            ok = pre_wait(s_full + tile, count[0]++ & 1, &s_abort, 42);
+            ok = mbar_wait(s_full + tile, count[0]++ & 1, &s_abort, 42);
             tc_fence_after();
           } else {
             ++count[1];
@@ -440,7 +416,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
               // the groups before are in O: those of earlier tiles are since there are scores of this one
-              if (half == 1) ok = ok && pre_wait(o_done + 2 * tile, (count[0] - 1) & 1, &s_abort, 43);
+              if (half == 1) ok = ok && mbar_wait(o_done + 2 * tile, (count[0] - 1) & 1, &s_abort, 43);
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -571,7 +547,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       const int stage = n % kPreStages;
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();
-      ok = pre_wait((values ? v_empty : k_empty) + stage, ((n / kPreStages) & 1) ^ 1, &s_abort, 45);
+      ok = mbar_wait((values ? v_empty : k_empty) + stage, ((n / kPreStages) & 1) ^ 1, &s_abort, 45);
       // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
       if (!values && lane == 0)
         reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(got_now);
@@ -624,7 +600,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       };
       auto values = [&](int t, uint32_t tile_number, int half, bool add) {
         const uint32_t va = base + L::kOffV + tile_number % kPreStages * L::kOperand + half * 8192;
-        ok = ok && pre_wait(p_full + 2 * t + half, p_phase[t][half]++ & 1, &s_abort, 51);
+        ok = ok && mbar_wait(p_full + 2 * t + half, p_phase[t][half]++ & 1, &s_abort, 51);
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
@@ -637,13 +613,13 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       for (;;) {
         const int rows = at.seq.n * a.g.G - at.rt * kPreRows, groups = pre_groups(a.c, at), tiles = (groups + 1) / 2;
         const bool two = rows > 128;
-        ok = ok && pre_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
-        ok = ok && pre_wait(q_full, q_phase[0]++ & 1, &s_abort, 47);
+        ok = ok && mbar_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
+        ok = ok && mbar_wait(q_full, q_phase[0]++ & 1, &s_abort, 47);
         if (!ok) break;
         tc_fence_after();
         scores(0, n, tiles == 1);
         if (two) {
-          ok = pre_wait(q_full + 1, q_phase[1]++ & 1, &s_abort, 48);
+          ok = mbar_wait(q_full + 1, q_phase[1]++ & 1, &s_abort, 48);
           if (!ok) break;
           tc_fence_after();
           scores(1, n, tiles == 1);
@@ -652,11 +628,11 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
 #pragma unroll 1
         for (int j = 0; j < tiles && ok; ++j, ++n) {
           const bool more = j + 1 < tiles, both = 2 * j + 1 < groups;
-          ok = pre_wait(v_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 50);
+          ok = mbar_wait(v_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 50);
           values(0, n, 0, j > 0);
           if (both) values(0, n, 1, true);
           if (more) {
-            ok = ok && pre_wait(k_full + (n + 1) % kPreStages, ((n + 1) / kPreStages) & 1, &s_abort, 52);
+            ok = ok && mbar_wait(k_full + (n + 1) % kPreStages, ((n + 1) / kPreStages) & 1, &s_abort, 52);
             if (!ok) break;
             tc_fence_after();
             scores(0, n + 1, j + 2 == tiles);
@@ -686,7 +662,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
 #pragma unroll 1
       for (int tile = 0; tile < (rows > 128 ? 2 : 1); ++tile) {
         const uint32_t use = uses[tile]++;
-        ok = ok && pre_wait(q_empty + tile, (use & 1) ^ 1, &s_abort, 55);
+        ok = ok && mbar_wait(q_empty + tile, (use & 1) ^ 1, &s_abort, 55);
         // 16-byte columns 2l and 2l + 1 of a row
         uint8_t* const dst = smem + L::kOffQ + tile * L::kOperand + (l >> 2) * L::kHalf;
         auto place = [&](int row, int c) { return dst + row * 128 + (((((2 * l) & 7) + c) ^ (row & 7)) << 4); };
