@@ -28,13 +28,14 @@ __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
 }
 
 // d / 16 lanes hold a head: lane l the elements 8l ... 8l + 7 of both halves, so that the rotation of positions, three
-// butterfly stages and the last one stay in registers.  A warp's heads belong to one token; a block takes TOKENS tokens of
-// the same heads, with the rows and the look-up of the sequence on their way at once.  grid: (T / TOKENS, pieces of 4 warps).
+// butterfly stages and the last one stay in registers.  A warp's heads belong to one token; its row and the look-up of its sequence
+// are on their way at once.  grid: (T, pieces of 4 warps).
 //
-// Bound by instructions for prompts (half of its issue slots go into the butterflies): all arithmetic on pairs, a - b as
-// fma(b, -1, a), the same number.  9937 tokens of 32 + 2 * 8 heads of 128: 86 us with scalars and a chain of four loads.
-template <int HD, int TOKENS>
-__global__ void __launch_bounds__(128)
+// Bound by instruction issue for prompts (two thirds of the slots, most of them butterflies and their shuffles): arithmetic on
+// pairs where that keeps every rounding, a - b as fma(b, -1, a).  9937 tokens of 32 + 2 * 8 heads of 128, 214 MB: 53 us; 86 with
+// scalars and a chain of four loads.  Twelve blocks an SM at 40 registers: two or four tokens a block took 3 and 12 us longer.
+template <int HD>
+__global__ void __launch_bounds__(128, 12)
 kv4_append_kernel(const __grid_constant__ Kv4Batch c, const unsigned short* qkv, int64_t ld, const float* cos_tab,
                   const float* sin_tab, int tab_rows, int hq, int rotate, unsigned short* __restrict__ q_out) {
   grid_dep_launch_dependents();
@@ -44,149 +45,140 @@ kv4_append_kernel(const __grid_constant__ Kv4Batch c, const unsigned short* qkv,
   const int head = blockIdx.y * (128 / LANES) + threadIdx.x / LANES, heads = hq + 2 * c.hkv;
   const bool live = head < heads;  // whole groups of lanes; the shuffles below want every lane
   const bool is_q = head < hq, is_v = head >= hq + c.hkv;
-  uint4 raw[TOKENS][2];
-#pragma unroll
-  for (int t = 0; t < TOKENS; ++t) {
-    const int row = blockIdx.x * TOKENS + t;
-    raw[t][0] = raw[t][1] = make_uint4(0, 0, 0, 0);
-    if (live && row < c.T) {
-      const unsigned short* src = qkv + row * ld + static_cast<int64_t>(head) * HD + 8 * l;
-      raw[t][0] = *reinterpret_cast<const uint4*>(src);
-      raw[t][1] = *reinterpret_cast<const uint4*>(src + HALF);
-    }
+  const int row = blockIdx.x;
+  uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (live) {
+    const unsigned short* src = qkv + row * ld + static_cast<int64_t>(head) * HD + 8 * l;
+    raw[0] = *reinterpret_cast<const uint4*>(src);
+    raw[1] = *reinterpret_cast<const uint4*>(src + HALF);
   }
   const float2 minus = make_float2(-1.0f, -1.0f);
+  int pos;
+  const int b = kv4_find(c, row, lane, &pos);
+  if (b >= c.B) return;
+  const bool there = pos >= 0 && pos < c.capacity && pos < tab_rows;
+  int page = -1;
+  if (there && !is_q) page = c.table[b * c.table_stride + (pos >> c.page_shift)];
+  float2 x[8];  // elements 8l + 2j, + 1 for j < 4, the same of the second half for j >= 4
+  {
+    const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
 #pragma unroll
-  for (int t = 0; t < TOKENS; ++t) {
-    const int row = blockIdx.x * TOKENS + t;
-    if (row >= c.T) return;
-    int pos;
-    const int b = kv4_find(c, row, lane, &pos);
-    if (b >= c.B) continue;
-    const bool there = pos >= 0 && pos < c.capacity && pos < tab_rows;
-    int page = -1;
-    if (there && !is_q) page = c.table[b * c.table_stride + (pos >> c.page_shift)];
-    float2 x[8];  // elements 8l + 2j, + 1 for j < 4, the same of the second half for j >= 4
-    {
-      const uint32_t w[8] = {raw[t][0].x, raw[t][0].y, raw[t][0].z, raw[t][0].w, raw[t][1].x, raw[t][1].y, raw[t][1].z, raw[t][1].w};
+    for (int j = 0; j < 8; ++j) x[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+  }
+  if (__any_sync(0xFFFFFFFFu, !is_v)) {
+    if (!is_v && there) {
+      const float4* cp = reinterpret_cast<const float4*>(cos_tab + static_cast<int64_t>(pos) * HALF + 8 * l);
+      const float4* sp = reinterpret_cast<const float4*>(sin_tab + static_cast<int64_t>(pos) * HALF + 8 * l);
+      const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
+      const float2 cs[4] = {make_float2(c0.x, c0.y), make_float2(c0.z, c0.w), make_float2(c1.x, c1.y), make_float2(c1.z, c1.w)};
+      const float2 sn[4] = {make_float2(s0.x, s0.y), make_float2(s0.z, s0.w), make_float2(s1.x, s1.y), make_float2(s1.z, s1.w)};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-    }
-    if (__any_sync(0xFFFFFFFFu, !is_v)) {
-      if (!is_v && there) {
-        const float4* cp = reinterpret_cast<const float4*>(cos_tab + static_cast<int64_t>(pos) * HALF + 8 * l);
-        const float4* sp = reinterpret_cast<const float4*>(sin_tab + static_cast<int64_t>(pos) * HALF + 8 * l);
-        const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
-        const float2 cs[4] = {make_float2(c0.x, c0.y), make_float2(c0.z, c0.w), make_float2(c1.x, c1.y), make_float2(c1.z, c1.w)};
-        const float2 sn[4] = {make_float2(s0.x, s0.y), make_float2(s0.z, s0.w), make_float2(s1.x, s1.y), make_float2(s1.z, s1.w)};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 a = x[j], d = x[j + 4];
-          // (scalars: packed products and sums were joined into packed FMAs, without the product's own rounding)
-          x[j] = make_float2(__fsub_rn(__fmul_rn(a.x, cs[j].x), __fmul_rn(d.x, sn[j].x)),
-                             __fsub_rn(__fmul_rn(a.y, cs[j].y), __fmul_rn(d.y, sn[j].y)));
-          x[j + 4] = make_float2(__fadd_rn(__fmul_rn(d.x, cs[j].x), __fmul_rn(a.x, sn[j].x)),
-                                 __fadd_rn(__fmul_rn(d.y, cs[j].y), __fmul_rn(a.y, sn[j].y)));
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = x[j], d = x[j + 4];
+        // (scalars: packed products and sums were joined into packed FMAs, without the product's own rounding)
+        x[j] = make_float2(__fsub_rn(__fmul_rn(a.x, cs[j].x), __fmul_rn(d.x, sn[j].x)),
+                           __fsub_rn(__fmul_rn(a.y, cs[j].y), __fmul_rn(d.y, sn[j].y)));
+        x[j + 4] = make_float2(__fadd_rn(__fmul_rn(d.x, cs[j].x), __fmul_rn(a.x, sn[j].x)),
+                               __fadd_rn(__fmul_rn(d.y, cs[j].y), __fmul_rn(a.y, sn[j].y)));
       }
-      if (rotate) {
-        // (value heads of a mixed warp take part in the shuffles and keep their own numbers)
-        float2 y[8];
+    }
+    if (rotate) {
+      // (value heads of a mixed warp take part in the shuffles and keep their own numbers)
+      float2 y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = make_float2(__fadd_rn(x[j].x, x[j].y), __fsub_rn(x[j].x, x[j].y));
+      for (int j = 0; j < 8; ++j) y[j] = make_float2(__fadd_rn(x[j].x, x[j].y), __fsub_rn(x[j].x, x[j].y));
 #pragma unroll
-        for (int h = 1; h < 4; h <<= 1)
+      for (int h = 1; h < 4; h <<= 1)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if ((j & h) == 0) {
-              const float2 u = y[j], w = y[j + h];
-              y[j] = __fadd2_rn(u, w);
-              y[j + h] = __ffma2_rn(w, minus, u);
-            }
-#pragma unroll
-        for (int h = 1; h < LANES; h <<= 1) {
-          const float sign = (l & h) ? -1.0f : 1.0f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 o = make_float2(__shfl_xor_sync(0xFFFFFFFFu, y[j].x, h), __shfl_xor_sync(0xFFFFFFFFu, y[j].y, h));
-            y[j] = __ffma2_rn(y[j], make_float2(sign, sign), o);
+        for (int j = 0; j < 8; ++j)
+          if ((j & h) == 0) {
+            const float2 u = y[j], w = y[j + h];
+            y[j] = __fadd2_rn(u, w);
+            y[j + h] = __ffma2_rn(w, minus, u);
           }
-        }
-        const float norm = HD == 128 ? 0.08838834764831845f : 0.125f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 u = y[j], w = y[j + 4];
-          y[j] = __fmul2_rn(__fadd2_rn(u, w), make_float2(norm, norm));
-          y[j + 4] = __fmul2_rn(__ffma2_rn(w, minus, u), make_float2(norm, norm));
-        }
-        if (!is_v) {
+      for (int h = 1; h < LANES; h <<= 1) {
+        const float sign = (l & h) ? -1.0f : 1.0f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = y[j];
+        for (int j = 0; j < 8; ++j) {
+          const float2 o = make_float2(__shfl_xor_sync(0xFFFFFFFFu, y[j].x, h), __shfl_xor_sync(0xFFFFFFFFu, y[j].y, h));
+          y[j] = __ffma2_rn(y[j], make_float2(sign, sign), o);
         }
       }
-    }
-    if (is_q && live) {
-      // a token without a place in the cache has no position: its query row is zero
-      uint32_t w[8];
+      const float norm = HD == 128 ? 0.08838834764831845f : 0.125f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = there ? bf16x2_of(x[j].x, x[j].y) : 0u;
-      unsigned short* dst = q_out + (static_cast<int64_t>(row) * hq + head) * HD + 8 * l;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-      *reinterpret_cast<uint4*>(dst + HALF) = make_uint4(w[4], w[5], w[6], w[7]);
+      for (int j = 0; j < 4; ++j) {
+        const float2 u = y[j], w = y[j + 4];
+        y[j] = __fmul2_rn(__fadd2_rn(u, w), make_float2(norm, norm));
+        y[j + 4] = __fmul2_rn(__ffma2_rn(w, minus, u), make_float2(norm, norm));
+      }
+      if (!is_v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = y[j];
+      }
     }
-    if (!__any_sync(0xFFFFFFFFu, live && !is_q)) continue;
-    // numbers that the grid cannot hold are rare: looked for in all of a warp's heads at once (0 * x is NaN for them, and fp16
-    // ends at 65504)
-    float2 odd = make_float2(0.0f, 0.0f);
-    float lo = x[0].x, hi = x[0].x;
+  }
+  if (is_q && live) {
+    // a token without a place in the cache has no position: its query row is zero
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = there ? bf16x2_of(x[j].x, x[j].y) : 0u;
+    unsigned short* dst = q_out + (static_cast<int64_t>(row) * hq + head) * HD + 8 * l;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + HALF) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  if (!__any_sync(0xFFFFFFFFu, live && !is_q)) return;
+  // numbers that the grid cannot hold are rare: looked for in all of a warp's heads at once (0 * x is NaN for them, and fp16
+  // ends at 65504)
+  float2 odd = make_float2(0.0f, 0.0f);
+  float lo = x[0].x, hi = x[0].x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    odd = __ffma2_rn(x[j], make_float2(0.0f, 0.0f), odd);
+    lo = fminf(lo, fminf(x[j].x, x[j].y));
+    hi = fmaxf(hi, fmaxf(x[j].x, x[j].y));
+  }
+  if (__any_sync(0xFFFFFFFFu, !(odd.x + odd.y == 0.0f) || lo < -65504.0f || hi > 65504.0f)) {
+    lo = 65504.0f, hi = -65504.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      odd = __ffma2_rn(x[j], make_float2(0.0f, 0.0f), odd);
+      x[j].x = isnan(x[j].x) ? 0.0f : fminf(fmaxf(x[j].x, -65504.0f), 65504.0f);
+      x[j].y = isnan(x[j].y) ? 0.0f : fminf(fmaxf(x[j].y, -65504.0f), 65504.0f);
       lo = fminf(lo, fminf(x[j].x, x[j].y));
       hi = fmaxf(hi, fmaxf(x[j].x, x[j].y));
     }
-    if (__any_sync(0xFFFFFFFFu, !(odd.x + odd.y == 0.0f) || lo < -65504.0f || hi > 65504.0f)) {
-      lo = 65504.0f, hi = -65504.0f;
+  }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j].x = isnan(x[j].x) ? 0.0f : fminf(fmaxf(x[j].x, -65504.0f), 65504.0f);
-        x[j].y = isnan(x[j].y) ? 0.0f : fminf(fmaxf(x[j].y, -65504.0f), 65504.0f);
-        lo = fminf(lo, fminf(x[j].x, x[j].y));
-        hi = fmaxf(hi, fmaxf(x[j].x, x[j].y));
-      }
-    }
+  for (int h = 1; h < LANES; h <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, h));
+    hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, h));
+  }
+  if (is_q || !live || static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.num_pages)) return;
+  const __half hs = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), hz = __float2half_rn(lo);
+  const float sf = __half2float(hs), zf = __half2float(hz);
+  const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
+  // rint and clamp as clamp and an addition whose sum has no room for a fraction; its bits are a constant plus the code, and
+  // the constants' sum is taken off the word at the end
+  uint32_t code[2] = {0, 0};
 #pragma unroll
-    for (int h = 1; h < LANES; h <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, h));
-      hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, h));
-    }
-    if (is_q || !live || static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.num_pages)) continue;
-    const __half hs = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), hz = __float2half_rn(lo);
-    const float sf = __half2float(hs), zf = __half2float(hz);
-    const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
-    // rint and clamp as clamp and an addition whose sum has no room for a fraction; its bits are a constant plus the code, and
-    // the constants' sum is taken off the word at the end
-    uint32_t code[2] = {0, 0};
+  for (int j = 0; j < 8; ++j) {
+    float2 r = __fmul2_rn(__fadd2_rn(x[j], make_float2(-zf, -zf)), make_float2(inv, inv));
+    r = make_float2(fminf(fmaxf(r.x, 0.0f), 15.0f), fminf(fmaxf(r.y, 0.0f), 15.0f));
+    r = __fadd2_rn(r, make_float2(12582912.0f, 12582912.0f));
+    code[j >> 2] += __float_as_uint(r.x) << (8 * (j & 3));
+    code[j >> 2] += __float_as_uint(r.y) << (8 * (j & 3) + 4);
+  }
+  uint32_t constants = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float2 r = __fmul2_rn(__fadd2_rn(x[j], make_float2(-zf, -zf)), make_float2(inv, inv));
-      r = make_float2(fminf(fmaxf(r.x, 0.0f), 15.0f), fminf(fmaxf(r.y, 0.0f), 15.0f));
-      r = __fadd2_rn(r, make_float2(12582912.0f, 12582912.0f));
-      code[j >> 2] += __float_as_uint(r.x) << (8 * (j & 3));
-      code[j >> 2] += __float_as_uint(r.y) << (8 * (j & 3) + 4);
-    }
-    uint32_t constants = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) constants += 0x4B400000u << (4 * j);
-    const int P = 1 << c.page_shift, slot = pos & (P - 1), kvh = head - hq - (is_v ? c.hkv : 0);
-    uint8_t* block = c.pages + page * c.page_stride + static_cast<int64_t>(kvh) * P * (HD + 8);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(block + (is_v ? P * HALF : 0) + slot * HALF) + l;
-    dst[0] = code[0] - constants;
-    dst[HALF / 8] = code[1] - constants;
-    if (l == 0) {
-      __half2* par = reinterpret_cast<__half2*>(block + P * HD + (is_v ? 4 * P : 0)) + slot;
-      *par = __halves2half2(hs, hz);
-    }
+  for (int j = 0; j < 8; ++j) constants += 0x4B400000u << (4 * j);
+  const int P = 1 << c.page_shift, slot = pos & (P - 1), kvh = head - hq - (is_v ? c.hkv : 0);
+  uint8_t* block = c.pages + page * c.page_stride + static_cast<int64_t>(kvh) * P * (HD + 8);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(block + (is_v ? P * HALF : 0) + slot * HALF) + l;
+  dst[0] = code[0] - constants;
+  dst[HALF / 8] = code[1] - constants;
+  if (l == 0) {
+    __half2* par = reinterpret_cast<__half2*>(block + P * HD + (is_v ? 4 * P : 0)) + slot;
+    *par = __halves2half2(hs, hz);
   }
 }
 
@@ -231,20 +223,6 @@ kv4_read_kernel(Kv4Batch c, unsigned short* __restrict__ k_out, unsigned short* 
   unsigned short* dst = (is_v ? v_out : k_out) + (static_cast<int64_t>(row) * c.hkv + kvh) * HD + 16 * l;
   reinterpret_cast<uint4*>(dst)[0] = o[0];
   reinterpret_cast<uint4*>(dst)[1] = o[1];
-}
-
-// One token a block until there are enough to fill the GPU twice over.
-template <int HD>
-static int launch_append(const Kv4Batch& c, const unsigned short* x, int64_t ld, const float* cos_tab, const float* sin_tab,
-                         int table_rows, int hq, int rotate, unsigned short* q, cudaStream_t s) {
-  const int pieces = (hq + 2 * c.hkv + 128 * 16 / HD - 1) / (128 * 16 / HD);
-  if (static_cast<int64_t>(c.T) * pieces < 4096)
-    DQ_CHECK_CUDA(launch_pdl(kv4_append_kernel<HD, 1>, dim3(c.T, pieces), dim3(128), 0, s, c, x, ld, cos_tab, sin_tab, table_rows,
-                             hq, rotate, q));
-  else
-    DQ_CHECK_CUDA(launch_pdl(kv4_append_kernel<HD, 2>, dim3((c.T + 1) / 2, pieces), dim3(128), 0, s, c, x, ld, cos_tab, sin_tab,
-                             table_rows, hq, rotate, q));
-  return DQ_OK;
 }
 
 int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out) {
@@ -312,8 +290,12 @@ extern "C" int dq_kv4_append(const dq_kv4_batch* batch, const void* qkv_bf16, in
   const auto* x = static_cast<const unsigned short*>(qkv_bf16);
   auto* q = static_cast<unsigned short*>(q_out_bf16);
   if (batch->head_dim == 128)
-    return launch_append<128>(c, x, ld_qkv, cos_tab, sin_tab, table_rows, hq, rotate, q, cs);
-  return launch_append<64>(c, x, ld_qkv, cos_tab, sin_tab, table_rows, hq, rotate, q, cs);
+    DQ_CHECK_CUDA(launch_pdl(kv4_append_kernel<128>, dim3(c.T, (heads + 15) / 16), dim3(128), 0, cs, c, x, ld_qkv, cos_tab,
+                             sin_tab, table_rows, hq, rotate, q));
+  else
+    DQ_CHECK_CUDA(launch_pdl(kv4_append_kernel<64>, dim3(c.T, (heads + 31) / 32), dim3(128), 0, cs, c, x, ld_qkv, cos_tab,
+                             sin_tab, table_rows, hq, rotate, q));
+  return DQ_OK;
 }
 
 extern "C" int dq_kv4_read(const dq_kv4_batch* batch, void* k_out_bf16, void* v_out_bf16, void* stream) {
