@@ -40,8 +40,7 @@ struct DecSmem {
   static constexpr int kOffMl = kOffMeet + kDecWarps * R * kPitch * 4;
   static constexpr int kQBytes = R * kQPitch<HD>;
   static constexpr int kOffQ = kOffMl + kDecWarps * R * 2 * 4;
-  static constexpr int kOffValid = kOffQ + kDecQueries * kQBytes;
-  static constexpr int kOffCursor = kOffValid + kDecWarps * kDecStages * 4;
+  static constexpr int kOffCursor = kOffQ + kDecQueries * kQBytes;
   static constexpr int kBytes = kOffCursor + static_cast<int>(sizeof(Kv4Cursor)) + 8;
   static_assert(kOffQ % 16 == 0 && kOffCursor % 4 == 0, "alignment");
 };
@@ -163,7 +162,6 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
   constexpr int R = L::R, MT = HD / 16, W = HD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * kDecStages * L::kStage;
-  uint32_t* valid = reinterpret_cast<uint32_t*>(smem + L::kOffValid) + warp * kDecStages;
   grid_dep_wait();
   // One warp looks up the CTA's share: its loads go to lines that every CTA wants at once.
   Kv4Cursor& found = *reinterpret_cast<Kv4Cursor*>(smem + L::kOffCursor);
@@ -183,8 +181,8 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
   Kv4Cursor ahead = at;  // where the copies are
   const int P = 1 << a.c.page_shift;
 
-  // A tile arrives in pieces of 16 tokens, each of one page: lane l copies every 32nd 16 bytes of the codes, lanes 0 to 7 the
-  // pairs.  The page of piece i is kept by lane i, one tile ahead.
+  // A tile arrives in pieces of 16 tokens, each of one page, or from one page: lane l copies every 32nd 16 bytes of the codes,
+  // lanes 0 to 7 the pairs of keys, 8 to 15 of values.  The page of piece i is kept by lane i, one tile ahead.
   bool more = true;
   int next_u = ahead.u0 + warp, next_page = -1, next_tok = 0;
   const uint8_t *src_codes = nullptr, *src_pairs = nullptr;  // the lane's 16 bytes of the head's block in page 0
@@ -194,7 +192,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
   auto seek_segment = [&]() {
     const uint8_t* block = a.c.pages + static_cast<int64_t>(ahead.h) * P * (HD + 8);
     src_codes = block + lane * 16;
-    src_pairs = block + P * HD + ((lane >> 2) & 1) * 4 * P + (lane & 3) * 16;
+    src_pairs = block + P * HD + ((lane >> 3) & 1) * 4 * P + (lane & 7) * 16;
     table_row = a.c.table + ahead.b * a.c.table_stride;
     there = min(ahead.seq.kv, a.c.capacity);
   };
@@ -228,39 +226,55 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     if (other) copy_queries();
   };
   const uint32_t dst_codes = smem_u32(ring) + lane * 16;
-  const uint32_t dst_pairs = smem_u32(ring) + kDecTile * HD + ((lane >> 2) & 1) * kDecTile * 4 + (lane & 3) * 16;
+  const uint32_t dst_pairs = smem_u32(ring) + kDecTile * HD + ((lane >> 3) & 1) * kDecTile * 4 + (lane & 7) * 16;
   const uint32_t page_bytes = static_cast<uint32_t>(a.c.page_stride);
-  auto fetch = [&](int stage) {
+  auto fetch = [&](int stage) {  // which pieces of the tile are there
+    uint32_t got = 0;
     if (more) {
-      const uint32_t got = __ballot_sync(0xFFFFFFFFu, static_cast<uint32_t>(next_page) < static_cast<uint32_t>(a.c.num_pages));
-      if (lane == 0) valid[stage] = got;
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const uint32_t page = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, next_page, i));
-        if ((got >> i) & 1u) {
-          const uint64_t off = static_cast<uint64_t>(page) * page_bytes;
-          const int slot = (next_tok + 16 * i) & (P - 1);
+      got = __ballot_sync(0xFFFFFFFFu, static_cast<uint32_t>(next_page) < static_cast<uint32_t>(a.c.num_pages));
+      if (P >= kDecTile) {  // one page
+        if (got & 1u) {
+          const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, next_page, 0))) * page_bytes;
+          const int slot = next_tok & (P - 1);
           const uint8_t* codes = src_codes + off + slot * (HD / 2);
-          const uint32_t to = dst_codes + stage * L::kStage + i * 16 * (HD / 2);
+          const uint32_t to = dst_codes + stage * L::kStage;
 #pragma unroll
-          for (int j = 0; j < HD / 64; ++j) {
+          for (int j = 0; j < HD / 32; ++j) {
             cp_async_16(to + j * 512, codes + j * 512);
             cp_async_16(to + kDecTile * (HD / 2) + j * 512, codes + P * (HD / 2) + j * 512);
           }
-          if (lane < 8) cp_async_16(dst_pairs + stage * L::kStage + i * 64, src_pairs + off + slot * 4);
+          if (lane < 16) cp_async_16(dst_pairs + stage * L::kStage, src_pairs + off + slot * 4);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const uint32_t page = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, next_page, i));
+          if ((got >> i) & 1u) {
+            const uint64_t off = static_cast<uint64_t>(page) * page_bytes;
+            const int slot = (next_tok + 16 * i) & (P - 1);
+            const uint8_t* codes = src_codes + off + slot * (HD / 2);
+            const uint32_t to = dst_codes + stage * L::kStage + i * 16 * (HD / 2);
+#pragma unroll
+            for (int j = 0; j < HD / 64; ++j) {
+              cp_async_16(to + j * 512, codes + j * 512);
+              cp_async_16(to + kDecTile * (HD / 2) + j * 512, codes + P * (HD / 2) + j * 512);
+            }
+            if ((lane & 7) < 4 && lane < 16) cp_async_16(dst_pairs + stage * L::kStage + i * 64, src_pairs + off + slot * 4);
+          }
         }
       }
       next_u += kDecWarps;
       seek();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");  // (an empty one too: groups are counted)
+    return got;
   };
   seek_segment();
   seek();
   copy_queries();
   asm volatile("cp.async.commit_group;" ::: "memory");
-#pragma unroll 1
-  for (int i = 0; i < kDecStages - 1; ++i) fetch(i);
+  static_assert(kDecStages == 2, "a tile is fetched while its predecessor is worked on");
+  uint32_t got_next = fetch(0);
   // the first segment's queries have arrived (the others': see kDecQueries)
   asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 1) : "memory");
   __syncthreads();
@@ -281,16 +295,17 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
       l[nt] = z[nt] = make_float2(0.0f, 0.0f);
     }
     const int kv = min(at.seq.kv, a.c.capacity);
+    // tiles from these tokens on are seen whole by every row
+    const int whole_hi = min(kv, at.span.p_lo + 1) - kDecTile, whole_lo = a.m.window > 0 ? at.span.p_hi - a.m.window : -1,
+              whole_sinks = a.m.window > 0 ? a.m.sinks - kDecTile : -1;
     for (int u = at.u0 + warp; u < at.u1; u += kDecWarps) {
       const uint8_t* buf = ring + stage * L::kStage;
       const int base = at.span.tile(u) * kDecTile;
-      fetch(stage == 0 ? kDecStages - 1 : stage - 1);  // into the tile that was read last
+      const uint32_t got = got_next;
+      got_next = fetch(stage ^ 1);  // into the tile that was read last
       asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 1) : "memory");
       __syncwarp();
-      const uint32_t got = valid[stage];
-      // every row sees every token of the tile?
-      const bool whole = got == (1u << kPieces) - 1 && base + kDecTile <= kv && base + kDecTile <= at.span.p_lo + 1 &&
-                         (a.m.window == 0 || base > at.span.p_hi - a.m.window || base + kDecTile <= a.m.sinks);
+      const bool whole = got == (1u << kPieces) - 1 && base <= whole_hi && (base > whole_lo || base <= whole_sinks);
       const __half2* kpar = reinterpret_cast<const __half2*>(buf + kDecTile * HD);
       const __half2* vpar = kpar + kDecTile;
       // S' = K Q': rows g and g + 8 are tokens.  Two chains of sums for each 16 tokens: a chain's products wait for one another
@@ -445,7 +460,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
           }
       }
       __syncwarp();  // every lane has read the tile
-      if (++stage == kDecStages) stage = 0;
+      stage ^= 1;
     }
     // the warps' sums meet
     float* meet = reinterpret_cast<float*>(smem + L::kOffMeet);
