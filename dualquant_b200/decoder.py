@@ -17,6 +17,9 @@ With tp > 1 the online Hadamards and the per-token activation scales are taken o
 own slice of the sharded axis (a valid rotation / scaling per shard, no collective); the only
 collectives are the two all-reduces per layer: NCCL in prefill; in decode either NCCL or, with
 fused_allreduce, a sum over NVLink peer memory inside the GEMM kernel's epilogue.
+
+The key/value cache is bf16 (torch's attention over it) or, with alloc_cache(..., kv="int4"), paged and 4 bits wide with this
+library's own append and attention kernels, optionally with a sliding window and first tokens that stay visible.
 """
 from __future__ import annotations
 
@@ -46,6 +49,17 @@ class DecoderConfig:
 
 
 LLAMA31_8B = DecoderConfig()
+
+
+@dataclass
+class PagedState:
+    """What the layers of a decoder share of its paged 4-bit cache."""
+
+    table: torch.Tensor  # int32 [batch, pages per sequence]
+    cos: torch.Tensor    # fp32 [positions, head_dim / 2]
+    sin: torch.Tensor
+    window: int = 0
+    sinks: int = 0
 
 
 class W4A4Linear:
@@ -164,20 +178,37 @@ class DecoderLayer:
         self.ln1 = torch.ones(cfg.hidden_size, dtype=torch.bfloat16, device=device)
         self.ln2 = torch.ones(cfg.hidden_size, dtype=torch.bfloat16, device=device)
         self.k_cache = self.v_cache = None
+        self.kv4: Optional[ops.KV4Cache] = None
+        self.paged: Optional[PagedState] = None
+
+    def alloc_paged(self, num_pages: int, page_size: int, state: PagedState, device):
+        self.k_cache = self.v_cache = None
+        self.kv4, self.paged = ops.kv4_cache(num_pages, self.hkv, self.cfg.head_dim, page_size, device), state
+
+    def attend_paged(self, qkv: torch.Tensor, kv_len: torch.Tensor) -> torch.Tensor:
+        """Append the new tokens of qkv [B * S, (hq + 2 hkv) * d] to the paged 4-bit cache and attend to it: [B * S, hq * d].
+        kv_len int32 [B]: tokens of each sequence with the new ones."""
+        st = self.paged
+        q = ops.kv4_append(qkv, st.cos, st.sin, self.kv4, st.table, kv_len, self.hq, rotate=self.cfg.online_hadamard)
+        return ops.kv4_attention(q, self.kv4, st.table, kv_len, window=st.window, sinks=st.sinks).flatten(1)
 
     def alloc_cache(self, batch: int, max_len: int, device):
+        self.kv4 = self.paged = None
         shape = (batch, self.hkv, max_len, self.cfg.head_dim)
         self.k_cache = torch.zeros(shape, dtype=torch.bfloat16, device=device)
         self.v_cache = torch.zeros(shape, dtype=torch.bfloat16, device=device)
 
     def forward(self, x, cos, sin, pos0: int, pos_t: Optional[torch.Tensor], mask, group, ar=None,
-                rope_tabs=None):
+                rope_tabs=None, kv_len: Optional[torch.Tensor] = None):
         """x [B, S, hidden] bf16.  Prefill: pos0 = 0, pos_t None (causal).  Decode: S = 1, the
-        cache position comes from the device tensor pos_t and `mask` hides the unwritten tail."""
+        cache position comes from the device tensor pos_t and `mask` hides the unwritten tail.
+        With a paged cache kv_len (int32 [B], tokens with the new ones) says all of that."""
         cfg = self.cfg
         B, S, Hd = x.shape
         hd = cfg.head_dim
         qkv = self.qkv.normed(x.reshape(B * S, Hd), self.ln1, cfg.rms_norm_eps)
+        if self.kv4 is not None:
+            return self._after_attention(x, self.attend_paged(qkv, kv_len), group, ar)
         if rope_tabs is not None:
             # RoPE + cache write in one launch; attention reads K / V straight from the cache
             if pos_t is not None:
@@ -212,7 +243,16 @@ class DecoderLayer:
         attn = attn.transpose(1, 2).reshape(B * S, self.hq * hd)
         return self._after_attention(x, attn, group, ar)
 
-    def forward_token_sharded(self, x, B: int, S: int, group, rope_tabs, codes, sx, xc=None):
+    def _prompt_attention(self, qkv, S: int, rope_tabs, kv_len):
+        """Attention of whole prompts, every token of qkv: [B * S, hq * d]."""
+        if self.kv4 is not None:
+            return self.attend_paged(qkv, kv_len)
+        q = ops.rope_kv_append(qkv, rope_tabs[0], rope_tabs[1], 0, self.hq, self.hkv, self.k_cache, self.v_cache, S)
+        attn = F.scaled_dot_product_attention(q, self.k_cache[:, :, :S], self.v_cache[:, :, :S], is_causal=True,
+                                              enable_gqa=True)
+        return attn.transpose(1, 2).reshape(qkv.shape[0], self.hq * self.cfg.head_dim)
+
+    def forward_token_sharded(self, x, B: int, S: int, group, rope_tabs, codes, sx, xc=None, kv_len=None):
         """Prompt pass under tensor parallelism with the residual stream sharded over tokens: x is
         this rank's [B * S / tp, hidden] slice (ranks own consecutive blocks of tokens).  RMSNorm
         and the activation quantiser run on the slice, the codes (one byte per element) and token
@@ -224,20 +264,14 @@ class DecoderLayer:
         row-parallel GEMMs push their output tiles into the owners' partial buffers from their
         epilogues, the owners add them onto x (in place) and push their codes to every rank."""
         if xc is not None:
-            return self._forward_token_sharded_peer(x, B, S, rope_tabs, xc)
+            return self._forward_token_sharded_peer(x, B, S, rope_tabs, xc, kv_len)
         cfg = self.cfg
         Tq, Hd = x.shape
-        T = B * S
-        hd = cfg.head_dim
         e4m3 = codes.dtype == torch.uint8
         c_sh, s_sh = ops.quant_act_int4_rmsnorm(x, self.ln1, cfg.rms_norm_eps, self.qkv.a, False, e4m3=e4m3)
         dist.all_gather_into_tensor(codes, c_sh, group=group)
         dist.all_gather_into_tensor(sx, s_sh, group=group)
-        qkv = self.qkv._gemm(codes, sx)
-        q = ops.rope_kv_append(qkv, rope_tabs[0], rope_tabs[1], 0, self.hq, self.hkv, self.k_cache, self.v_cache, S)
-        attn = F.scaled_dot_product_attention(q, self.k_cache[:, :, :S], self.v_cache[:, :, :S], is_causal=True,
-                                              enable_gqa=True)
-        o = self.o(attn.transpose(1, 2).reshape(T, self.hq * hd))
+        o = self.o(self._prompt_attention(self.qkv._gemm(codes, sx), S, rope_tabs, kv_len))
         o_sh = torch.empty(Tq, Hd, dtype=o.dtype, device=o.device)
         dist.reduce_scatter_tensor(o_sh, o, group=group)
         x = x + o_sh
@@ -250,17 +284,12 @@ class DecoderLayer:
         dist.reduce_scatter_tensor(d_sh, d, group=group)
         return x + d_sh
 
-    def _forward_token_sharded_peer(self, x, B: int, S: int, rope_tabs, xc):
+    def _forward_token_sharded_peer(self, x, B: int, S: int, rope_tabs, xc, kv_len=None):
         cfg = self.cfg
-        T = B * S
         c_sh, s_sh = ops.quant_act_int4_rmsnorm(x, self.ln1, cfg.rms_norm_eps, self.qkv.a, False, e4m3=True)
         xc.push(c_sh, s_sh)
         xc.barrier()  # every rank's codes have landed here
-        qkv = self.qkv._gemm(xc.codes, xc.sx)
-        q = ops.rope_kv_append(qkv, rope_tabs[0], rope_tabs[1], 0, self.hq, self.hkv, self.k_cache, self.v_cache, S)
-        attn = F.scaled_dot_product_attention(q, self.k_cache[:, :, :S], self.v_cache[:, :, :S], is_causal=True,
-                                              enable_gqa=True)
-        attn = attn.transpose(1, 2).reshape(T, self.hq * cfg.head_dim)
+        attn = self._prompt_attention(self.qkv._gemm(xc.codes, xc.sx), S, rope_tabs, kv_len)
         c_o, s_o = ops.quant_act_int4(attn, self.o.a, self.o.had, False, e4m3=True)
         ops.gemm_w4a4_int4_e4m3_scatter(c_o, s_o, self.o.pw.bytes_e4m3(), self.o.pw, self.o.r, xc)
         xc.barrier()  # every rank's partial rows for this rank's tokens have landed
@@ -331,17 +360,43 @@ class Decoder:
         self.norm = torch.ones(cfg.hidden_size, dtype=torch.bfloat16, device=device)
         self.layers = [DecoderLayer(cfg, tp, device, gen, keep_codes, shared) for _ in range(cfg.num_hidden_layers)]
         self.max_len = 0
+        self.paged: Optional[PagedState] = None
 
-    def alloc_cache(self, batch: int, max_len: int):
+    def alloc_cache(self, batch: int, max_len: int, kv: str = "bf16", page_size: int = 64, window: int = 0, sinks: int = 0):
+        """kv: "bf16" - dense bf16 caches; "int4" - pages of page_size tokens, 4 bits per element (head_dim 64 or 128), with an
+        optional sliding window and first tokens that stay visible (ops.kv4_attention)."""
+        if kv not in ("bf16", "int4"):
+            raise ValueError("kv must be 'bf16' or 'int4'")
+        if kv == "bf16" and (window or sinks):
+            raise ValueError("a window and sinks need the paged cache (kv='int4')")
         self.max_len = max_len
-        for layer in self.layers:
-            layer.alloc_cache(batch, max_len, self.device)
+        self.paged = None
+        if kv == "int4":
+            per_seq = -(-max_len // page_size)
+            table = torch.arange(batch * per_seq, dtype=torch.int32, device=self.device).view(batch, per_seq)
+            d = self.cfg.head_dim
+            inv = self.cfg.rope_theta ** -(torch.arange(0, d, 2, device=self.device, dtype=torch.float64) / d)
+            ang = torch.arange(max_len, device=self.device, dtype=torch.float64)[:, None] * inv[None, :]
+            self.paged = PagedState(table, ang.cos().float(), ang.sin().float(), window, sinks)
+            for layer in self.layers:
+                layer.alloc_paged(batch * per_seq, page_size, self.paged, self.device)
+        else:
+            for layer in self.layers:
+                layer.alloc_cache(batch, max_len, self.device)
         self.cos, self.sin = _rope_tables(self.cfg, max_len, self.device)
 
-    def prefill(self, ids: torch.Tensor) -> torch.Tensor:
-        """ids [B, S] -> logits of the last position [B, vocab]."""
+    def _kv_len(self, batch: int, n: int) -> Optional[torch.Tensor]:
+        return None if self.paged is None else torch.full((batch,), n, dtype=torch.int32, device=self.device)
+
+    def prefill(self, ids: torch.Tensor, pos0: int = 0) -> torch.Tensor:
+        """ids [B, S] -> logits of the last position [B, vocab].  pos0 (paged cache): the tokens follow pos0 tokens that the
+        cache holds already, the next piece of a prompt."""
         B, S = ids.shape
-        return self._prefill_tail(self._prefill_body(ids), B, S)
+        if pos0 and self.paged is None:
+            raise ValueError("prompts in pieces need the paged cache (kv='int4')")
+        if pos0 < 0 or pos0 + S > self.max_len:
+            raise ValueError(f"positions {pos0} .. {pos0 + S - 1} outside of the cache of {self.max_len}")
+        return self._prefill_tail(self._prefill_body(ids, pos0), B, S)
 
     def _token_sharded(self, B: int, S: int) -> bool:
         return self.tp > 1 and self.token_sharded_prefill and (B * S) % self.tp == 0
@@ -350,18 +405,19 @@ class Decoder:
         return (self._token_sharded(B, S) and self.prefill_exchange == "peer" and
                 sharding.peer_exchange_fits(B * S, self.tp, self.cfg.hidden_size))
 
-    def _prefill_body(self, ids: torch.Tensor) -> torch.Tensor:
+    def _prefill_body(self, ids: torch.Tensor, pos0: int = 0) -> torch.Tensor:
         """The decoder layers of a prompt pass: kernels on the current stream only - no host
         synchronisation and, on one GPU or with the peer-memory exchange, no library collective - so
         that it can be captured in a CUDA graph.  Returns the last positions' hidden states [B, hidden]
         or, token-sharded, this rank's slice of the residual stream."""
         cfg = self.cfg
         B, S = ids.shape
+        kv_len = self._kv_len(B, pos0 + S)
         if not self._token_sharded(B, S):
             x = self.embed[ids]
             cos, sin = self.cos[:S], self.sin[:S]
             for layer in self.layers:
-                x = layer.forward(x, cos, sin, 0, None, None, self.group, rope_tabs=(self.cos, self.sin))
+                x = layer.forward(x, cos, sin, 0, None, None, self.group, rope_tabs=(self.cos, self.sin), kv_len=kv_len)
             return x[:, -1]
         T, Hd = B * S, cfg.hidden_size
         lo, hi = sharding.token_shard(T, self.tp, self.rank)
@@ -380,7 +436,7 @@ class Decoder:
             codes = torch.empty(T, Hd, dtype=torch.uint8 if e4m3 else torch.int8, device=self.device)
             sx = torch.empty(T, dtype=torch.float32, device=self.device)
         for layer in self.layers:
-            x = layer.forward_token_sharded(x, B, S, self.group, (self.cos, self.sin), codes, sx, xc)
+            x = layer.forward_token_sharded(x, B, S, self.group, (self.cos, self.sin), codes, sx, xc, kv_len)
         return x
 
     def _prefill_tail(self, x: torch.Tensor, B: int, S: int) -> torch.Tensor:
@@ -437,6 +493,12 @@ class Decoder:
         """ids [B] (one token per sequence), pos_t: int64 device tensor [1] with the cache position.
         Everything is indexed through pos_t, so the step can be captured in a CUDA graph."""
         x = self.embed[ids].unsqueeze(1)
+        if self.paged is not None:
+            kv_len = (pos_t + 1).to(torch.int32).expand(ids.shape[0]).contiguous()
+            for layer in self.layers:
+                x = layer.forward(x, None, None, 0, pos_t, None, self.group, self.ar, kv_len=kv_len)
+            x = _rms_norm(x[:, 0], self.norm, self.cfg.rms_norm_eps)
+            return x @ self.lm_head.T
         cos = self.cos.index_select(0, pos_t)
         sin = self.sin.index_select(0, pos_t)
         # additive mask over the unwritten tail of the cache, built once per step (a boolean mask
