@@ -35,11 +35,15 @@ template <int HD, int NT>
 struct DecSmem {
   static constexpr int R = 8 * NT;
   static constexpr int kStage = kDecTile * (HD + 8);
-  static constexpr int kPitch = HD + 8;  // floats per row of a warp's output in the meeting place
-  static constexpr int kOffMeet = kDecWarps * kDecStages * kStage;
-  static constexpr int kOffMl = kOffMeet + kDecWarps * R * kPitch * 4;
+  // Where the warps' outputs meet: up to eight rows in the half of a warp's ring that it fills next, sixteen in a place of
+  // their own.
+  static constexpr int kPitch = HD + 8;  // floats per row
+  static constexpr int kRing = kDecWarps * kDecStages * kStage;
+  static constexpr bool kMeetInRing = R * kPitch * 4 <= kStage;
+  static constexpr int kOffMl = kRing + (kMeetInRing ? 0 : kDecWarps * R * kPitch * 4);
   static constexpr int kQBytes = R * kQPitch<HD>;
-  static constexpr int kOffQ = kOffMl + kDecWarps * R * 2 * 4;
+  static constexpr int kOffHalf = kOffMl + kDecWarps * R * 2 * 4;
+  static constexpr int kOffQ = kOffHalf + 16;
   static constexpr int kOffCursor = kOffQ + kDecQueries * kQBytes;
   static constexpr int kBytes = kOffCursor + static_cast<int>(sizeof(Kv4Cursor)) + 8;
   static_assert(kOffQ % 16 == 0 && kOffCursor % 4 == 0, "alignment");
@@ -463,8 +467,14 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
       stage ^= 1;
     }
     // the warps' sums meet
-    float* meet = reinterpret_cast<float*>(smem + L::kOffMeet);
+    // (a warp's tiles in flight are in half `stage` of its ring, and the halves change alike or not at all: the others' are told)
+    auto meet_of = [&](int w, int free_half) {
+      return reinterpret_cast<float*>(smem + (L::kMeetInRing ? (w * kDecStages + free_half) * L::kStage
+                                                             : L::kRing + w * R * L::kPitch * 4));
+    };
+    float* const mine = meet_of(warp, stage ^ 1);
     float* ml = reinterpret_cast<float*>(smem + L::kOffMl);
+    int* half_of = reinterpret_cast<int*>(smem + L::kOffHalf);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -476,7 +486,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
           zs += __shfl_xor_sync(0xFFFFFFFFu, zs, d);
         }
         const int r = nt * 8 + 2 * t + i;
-        float* dst = meet + (warp * R + r) * L::kPitch + g * (2 * MT);
+        float* dst = mine + r * L::kPitch + g * (2 * MT);
 #pragma unroll
         for (int j = 0; j < MT / 2; ++j)
           reinterpret_cast<float4*>(dst)[j] =
@@ -487,6 +497,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
           ml[(warp * R + r) * 2 + 1] = ls;
         }
       }
+    if (lane == 0) half_of[warp] = stage ^ 1;
     __syncthreads();
     const int rows = min(R, at.seq.n * a.g.G - at.rt * R);
     const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
@@ -512,7 +523,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
       for (int w = 0; w < kDecWarps; ++w) {
         const float by = exp2_approx(ml[(w * R + r) * 2] - top);
         sum = fmaf(by, ml[(w * R + r) * 2 + 1], sum);
-        acc = fmaf(by, meet[(w * R + r) * L::kPitch + d], acc);
+        acc = fmaf(by, meet_of(w, half_of[w])[r * L::kPitch + d], acc);
       }
       if (whole_segment) {
         const int at_row = at.rt * R + r, i = a.g.by(at_row), head = at.h * a.g.G + (at_row - i * a.g.G);
