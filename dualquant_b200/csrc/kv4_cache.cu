@@ -6,9 +6,10 @@
 //   lo = x1 c - x2 s, hi = x2 c + x1 s        x1, x2: the halves of the head; each product and sum rounded on its own
 //   butterflies h = 1, 2, 4 ... d / 2, then times fp32(d^-1/2)
 //   scale = fp16((max - min) * fp32(1 / 15)), zero = fp16(min), code = clamp(rint((x - zero) * (1 / scale)), 0, 15)
+//   (one step of fp16 less scale where 15 scale + zero would round to infinity there: only heads that reach past 65400)
 // The two roundings to fp16 are the storage of the grid: codes are taken on the stored grid, and 4 bytes a head against
 // d / 2 of codes are 6 to 12 % of the cache.  NaN is stored as 0 and what fp16 cannot hold as +-65504, so that a page that
-// was written holds finite numbers only.
+// was written stands for finite numbers only, in fp16 too (the keys and values of kv4_prefill_kernel).
 #include "kv4.cuh"
 
 namespace dq {
@@ -154,7 +155,10 @@ kv4_append_kernel(const __grid_constant__ Kv4Batch c, const unsigned short* qkv,
     hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, h));
   }
   if (is_q || !live || static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.num_pages)) return;
-  const __half hs = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), hz = __float2half_rn(lo);
+  __half hs = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+  const __half hz = __float2half_rn(lo);
+  // 15 scale + zero is at most 65504 + 16 (zero) + 7.5 ulp (scale), and 65520 is the first that rounds to infinity
+  if (fmaf(15.0f, __half2float(hs), __half2float(hz)) >= 65520.0f) hs = __ushort_as_half(__half_as_ushort(hs) - 1);
   const float sf = __half2float(hs), zf = __half2float(hz);
   const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
   // rint and clamp as clamp and an addition whose sum has no room for a fraction; its bits are a constant plus the code, and

@@ -696,5 +696,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, k
     """Causal grouped-query attention of the new tokens (q [T, hq, d] bf16, rows as in kv4_append) over the paged 4-bit cache:
     bf16 [T, hq, d].  window > 0: a token sees itself, the window - 1 tokens before it and the first `sinks` tokens of its
     sequence.  scale: default d ** -0.5.  max_new: the most rows that a sequence brings, which chooses the kernel; T (or T / B
-    without cu_new) if not given.  A row that sees no token is zero; rows from cu_new[B] on are not written."""
+    without cu_new) if not given.  A row that sees no token is zero; rows from cu_new[B] on are not written.  With more than 32
+    rows to a key/value head (hq / hkv * max_new) keys and values are rounded to fp16 (2^-11 of the number), with fewer the
+    products are taken of the codes themselves."""
     return _lib.host().kv4_attention(q, cache, block_table, kv_len, cu_new, max_new, window, sinks, scale, out)

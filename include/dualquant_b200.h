@@ -612,7 +612,8 @@ typedef struct dq_kv4_batch {
 DQ_API size_t dq_kv4_page_bytes(int hkv, int head_dim, int page_size);
 /* New tokens into the cache: qkv [tokens][(hq + 2 hkv) * head_dim] bf16; position rotation of query and key heads from fp32
  * tables [table_rows][head_dim / 2], with rotate != 0 a normalised Walsh-Hadamard rotation of both over the head, 4-bit
- * quantisation of keys and values (scale fp16((max - min) / 15), zero fp16(min); NaN as 0, +-65504 at most).  q_out
+ * quantisation of keys and values (scale fp16((max - min) / 15), a step of fp16 less where 15 scale + zero would be infinite in
+ * fp16, zero fp16(min); NaN as 0, +-65504 at most).  q_out
  * [tokens][hq][head_dim] bf16 gets the rotated queries.  A token whose position is negative, behind the table row or behind
  * the rotation tables is not written and has a zero query row; one whose page is not there is not written. */
 DQ_API int dq_kv4_append(const dq_kv4_batch* batch, const void* qkv_bf16, int64_t ld_qkv, const float* cos_tab,
@@ -622,7 +623,9 @@ DQ_API int dq_kv4_read(const dq_kv4_batch* batch, void* k_out_bf16, void* v_out_
 /* Causal attention of the new tokens over the cache: hq query heads in groups of hq / hkv, q [tokens][hq][head_dim] bf16 with
  * the given strides (elements).  window > 0: a token sees itself, the window - 1 tokens before it and the first `sinks`
  * tokens of its sequence.  max_new: no sequence brings more rows (a hint; more are computed all the same).  A row that sees
- * nothing is zero.  out [tokens][hq][head_dim] bf16. */
+ * nothing is zero.  out [tokens][hq][head_dim] bf16.  Groups of up to 32 rows (hq / hkv * max_new) multiply with the codes
+ * themselves; with more rows keys and values are scale * c + zero rounded to fp16 (2^-11 of the number).  cu_new must not
+ * decrease: of a batch in which it does, rows may be left out. */
 DQ_API size_t dq_kv4_attention_workspace_bytes(const dq_kv4_batch* batch, int hq, int max_new);
 DQ_API int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, int64_t q_row_stride, int64_t q_head_stride,
                             int hq, int max_new, int window, int sinks, float scale, void* out_bf16, void* workspace,

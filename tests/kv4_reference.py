@@ -82,6 +82,8 @@ def quantise(x):
     x = torch.where(x.isnan(), torch.zeros_like(x), x).clamp(-65504.0, 65504.0)
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
     s, z = ((hi - lo) * (1.0 / 15.0)).half(), lo.half()
+    # a grid that passes what fp16 holds (15 s + z rounds to infinity from 65520 on): one step of fp16 less
+    s = torch.where(15 * s.double() + z.double() >= 65520, (s.view(torch.int16) - 1).view(torch.float16), s)
     inv = torch.where(s > 0, 1.0 / s.float(), torch.zeros_like(lo))
     return ((x - z.float()) * inv).round().clamp(0, 15), s, z
 

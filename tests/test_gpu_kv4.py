@@ -526,3 +526,72 @@ def test_offsets_that_pass_32_bits():
     assert bool(((got.double() - want).abs() <= ref.attention_tolerance(want, vs, [page * 3])).all())
     k, v = ops.kv4_read(cache, far, n, 1)
     assert bool(((k[0].double() - ks[0][:, -1]).abs() <= 2.0 ** -8 * ks[0][:, -1].abs() + 1e-5).all())
+
+
+def test_heads_up_to_the_largest_number_of_fp16_stay_finite_where_they_are_seen_and_where_not():
+    # 65504 / 15 rounds up to 4368, and 15 * 4368 = 65520 would be infinite in fp16: zero weights times it would not be zero
+    hq, hkv, hd, page, n = 2, 1, 64, 16, 80
+    x = torch.zeros(n, 4 * hd)
+    x[:, :hd] = torch.randn(n, hd, generator=torch.Generator().manual_seed(5))
+    x[n - 1, 2 * hd + 3] = 65280.0  # key and value of the last token: only it sees them
+    x[n - 1, 3 * hd + 1] = float("inf")
+    x = x.to(torch.bfloat16).cuda()
+    cos, sin = torch.ones(n, hd // 2).cuda(), torch.zeros(n, hd // 2).cuda()
+    cache = ops.kv4_cache(5, hkv, hd, page)
+    table, length = i32([[3, 1, 4, 0, 2]]), i32([n])
+    q = ops.kv4_append(x, cos, sin, cache, table, length, hq, rotate=False)
+    _, kp, vc, vp = ref.unpack(cache.pages, table, [n], hkv, hd, page)[0]
+    got = 15 * vp[n - 1, 0, 0].double() + vp[n - 1, 0, 1].double()
+    assert 65400 < float(got) <= 65504 and int(vc[n - 1, 0, 1]) == 15
+    assert bool((15 * kp[..., 0].double() + kp[..., 1].double() < 65520).all())
+    for most in (1, n):
+        out = ops.kv4_attention(q, cache, table, length, max_new=most)
+        assert bool(out.isfinite().all()) and bool((out[: n - 1] == 0).all())
+
+
+def test_calls_back_to_back_on_one_and_on_two_streams_give_the_same_bits():
+    # nothing waits for a call before the next: barriers, workspaces and joins of neighbouring calls must not meet
+    gen = torch.Generator().manual_seed(11)
+    batches = []
+    for new, lengths, heads in (([300, 0, 17, 128], [1700, 0, 900, 128], (8, 2, 128)), ([1] * 40, list(range(1, 4001, 100)), (8, 1, 64)),
+                                ([4, 2, 9], [3000, 77, 2000], (4, 4, 128)), ([700], [700], (4, 1, 64))):
+        hq, hkv, hd = heads
+        pages, table, _, _ = ref.make_cache(gen, len(new), lengths, hkv, hd, 32)
+        q = torch.randn(sum(new), hq, hd, generator=gen).to(torch.bfloat16).cuda()
+        args = (q, ops.KV4Cache(pages, hd, 32), table, i32(lengths), cu_of(new), max(new))
+        batches.append((args, ops.kv4_attention(*args).clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i in range(200):
+        args, want = batches[i % len(batches)]
+        with torch.cuda.stream(streams[(i // 3) % 2 if i >= 100 else 0]):
+            got.append((ops.kv4_attention(*args), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in got)
+
+
+@pytest.mark.parametrize("most", [1, 200])
+def test_row_offsets_that_decrease_touch_nothing_else(most):
+    gen = torch.Generator().manual_seed(12)
+    pages, table, ks, vs = ref.make_cache(gen, 3, [300, 200, 300], 2, 128, 16)
+    q = torch.randn(260, 4, 128, generator=gen).to(torch.bfloat16).cuda()
+    cache, length = ops.KV4Cache(pages, 128, 16), i32([300, 200, 300])
+    out = torch.full((260, 4, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv4_attention(q, cache, table, length, i32([0, 200, 100, 250]), most, out=out)
+    assert bool((out[250:] == 7).all())
+    out = ops.kv4_attention(q, cache, table, length, cu_of([100, 100, 60]), most)
+    want = ref.attention(q, ks, vs, [100, 100, 60], [300, 200, 300])
+    assert bool(((out.double() - want).abs() <= ref.attention_tolerance(want, vs, [300])).all())
+
+
+@pytest.mark.parametrize("B,new", [(33, 1), (128, 2), (129, 1), (300, 3), (40, 40)])
+def test_batches_of_more_sequences_than_lanes(B, new):
+    gen = torch.Generator().manual_seed(B)
+    lengths = [0 if b % 7 == 3 else new + (b * 37) % 150 for b in range(B)]
+    rows = [0 if m == 0 else new for m in lengths]
+    pages, table, ks, vs = ref.make_cache(gen, B, lengths, 1, 64, 16)
+    q = torch.randn(sum(rows), 2, 64, generator=gen).to(torch.bfloat16).cuda()
+    out = ops.kv4_attention(q, ops.KV4Cache(pages, 64, 16), table, i32(lengths), cu_of(rows), new)
+    want = ref.attention(q, ks, vs, rows, lengths)
+    assert bool(((out.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths)).all())
