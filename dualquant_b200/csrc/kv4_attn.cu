@@ -118,6 +118,9 @@ struct Kv4Plan {
 static Kv4Plan kv4_plan(const Kv4Batch& c, int G, int hd, int max_new, DeviceState* st) {
   Kv4Plan p;
   const int64_t rows = static_cast<int64_t>(G) * max_new;
+  // The few-rows kernel reads the cache once for every 16 rows, the other one takes up to 256 at the cost of one.  32 heads of
+  // 128 over 8, us, few / many: 16 rows over 16 x 4000 tokens 36 / 69, over 8 x 30000 83 / 215; 32 rows 58 / 70, 150 / 216 (and
+  // 20 / 16 over 1 x 4000); 48 rows 82 / 71, 219 / 217; 64 rows 100 / 72, 286 / 218.
   p.R = rows <= 8 ? 8 : rows <= 32 ? 16 : kPreRows;
   const int tile = p.R == kPreRows ? kPreTile : kDecTile, least = p.R == kPreRows ? kPreLeast : kDecLeast;
   const int64_t row_tiles = (static_cast<int64_t>(c.T) * G + p.R - 1) / p.R + c.B;

@@ -186,11 +186,39 @@ kv4_append_kernel(const __grid_constant__ Kv4Batch c, const unsigned short* qkv,
   }
 }
 
-// The values of the last n tokens of each sequence as bf16 rows.  A lane makes 16 elements of a key or value head.
-// Rows of tokens that the cache does not hold are zero.  grid: (T, pieces of 128 threads over 2 * hkv * d / 16 lanes).
+// Eight codes of a word as 2^23 + c 16^k with k such that the code stays where it is in the mantissa: one logic operation each
+// (and a shift for the last three), then exact arithmetic on pairs.  -> bf16 of c * scale + zero, one rounding each
+struct Kv4Grid {
+  float2 by[3];  // scale / 16^k of codes 2j and 2j + 1: (k = 0, 1), (2, 3), (4, 2)
+  float2 zero;
+};
+__device__ __forceinline__ Kv4Grid kv4_grid(__half2 pair) {
+  const float2 f = __half22float2(pair);
+  Kv4Grid r;
+  r.by[0] = make_float2(f.x, f.x * 0.0625f);
+  r.by[1] = make_float2(f.x * 0.00390625f, f.x * 0.000244140625f);
+  r.by[2] = make_float2(f.x * 0.0000152587890625f, r.by[1].x);
+  r.zero = make_float2(f.y, f.y);
+  return r;
+}
+__device__ __forceinline__ uint4 kv4_values(uint32_t w, const Kv4Grid& g) {
+  constexpr uint32_t k23 = 0x4B000000u;
+  const float2 off = make_float2(-8388608.0f, -8388608.0f);
+  const uint32_t v = w >> 12;  // codes 5, 6, 7 at k = 2, 3, 4
+  auto at = [](uint32_t x, int k) { return __uint_as_float((x & (15u << (4 * k))) | k23); };
+  auto pair = [&](float lo, float hi, float2 by) {
+    const float2 x = __ffma2_rn(__fadd2_rn(make_float2(lo, hi), off), by, g.zero);
+    return bf16x2_of(x.x, x.y);
+  };
+  return make_uint4(pair(at(w, 0), at(w, 1), g.by[0]), pair(at(w, 2), at(w, 3), g.by[1]), pair(at(w, 4), at(v, 2), g.by[2]),
+                    pair(at(v, 3), at(v, 4), make_float2(g.by[1].y, g.by[2].x)));
+}
+
+// The values of the last n tokens of each sequence as bf16 rows.  A lane makes 16 elements of a key head and 16 of the value head
+// beside it.  Rows of tokens that the cache does not hold are zero.  grid: (T, pieces of 64 threads over hkv * d / 16 lanes).
 template <int HD>
-__global__ void __launch_bounds__(128)
-kv4_read_kernel(Kv4Batch c, unsigned short* __restrict__ k_out, unsigned short* __restrict__ v_out) {
+__global__ void __launch_bounds__(64)
+kv4_read_kernel(const __grid_constant__ Kv4Batch c, unsigned short* __restrict__ k_out, unsigned short* __restrict__ v_out) {
   grid_dep_launch_dependents();
   grid_dep_wait();
   constexpr int LANES = HD / 16;
@@ -198,35 +226,27 @@ kv4_read_kernel(Kv4Batch c, unsigned short* __restrict__ k_out, unsigned short* 
   int pos;
   const int b = kv4_find(c, row, lane, &pos);
   if (b >= c.B) return;
-  const int unit = blockIdx.y * 128 + threadIdx.x, head = unit / LANES, l = unit % LANES;
-  if (head >= 2 * c.hkv) return;
-  const bool is_v = head >= c.hkv;
-  const int kvh = head - (is_v ? c.hkv : 0);
+  const int unit = blockIdx.y * 64 + threadIdx.x, head = unit / LANES, l = unit % LANES;
+  if (head >= c.hkv) return;
   const int P = 1 << c.page_shift, slot = pos & (P - 1);
-  uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  uint4 k[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, v[2] = {k[0], k[0]};
   int page = -1;
   if (pos >= 0 && pos < c.capacity) page = c.table[b * c.table_stride + (pos >> c.page_shift)];
-  if (page >= 0 && page < c.num_pages) {
-    const uint8_t* block = c.pages + page * c.page_stride + static_cast<int64_t>(kvh) * P * (HD + 8);
-    const uint2 w = *reinterpret_cast<const uint2*>(block + (is_v ? P * HD / 2 : 0) + slot * (HD / 2) + 8 * l);
-    const float2 sz = __half22float2(*(reinterpret_cast<const __half2*>(block + P * HD + (is_v ? 4 * P : 0)) + slot));
-    const uint32_t word[2] = {w.x, w.y};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t r[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // (the product is exact, so contraction into one FMA changes nothing)
-        const float a = static_cast<float>((word[i] >> (8 * j)) & 15u) * sz.x + sz.y;
-        const float d = static_cast<float>((word[i] >> (8 * j + 4)) & 15u) * sz.x + sz.y;
-        r[j] = bf16x2_of(a, d);
-      }
-      o[i] = make_uint4(r[0], r[1], r[2], r[3]);
-    }
+  if (static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages)) {
+    const uint8_t* block = c.pages + page * c.page_stride + static_cast<int64_t>(head) * P * (HD + 8);
+    const uint8_t *codes = block + slot * (HD / 2) + 8 * l, *pairs = block + P * HD + 4 * slot;
+    const uint2 kw = *reinterpret_cast<const uint2*>(codes), vw = *reinterpret_cast<const uint2*>(codes + P * (HD / 2));
+    const Kv4Grid kg = kv4_grid(*reinterpret_cast<const __half2*>(pairs)), vg = kv4_grid(*reinterpret_cast<const __half2*>(pairs + 4 * P));
+    k[0] = kv4_values(kw.x, kg);
+    k[1] = kv4_values(kw.y, kg);
+    v[0] = kv4_values(vw.x, vg);
+    v[1] = kv4_values(vw.y, vg);
   }
-  unsigned short* dst = (is_v ? v_out : k_out) + (static_cast<int64_t>(row) * c.hkv + kvh) * HD + 16 * l;
-  reinterpret_cast<uint4*>(dst)[0] = o[0];
-  reinterpret_cast<uint4*>(dst)[1] = o[1];
+  const int64_t to = (static_cast<int64_t>(row) * c.hkv + head) * HD + 16 * l;
+  reinterpret_cast<uint4*>(k_out + to)[0] = k[0];
+  reinterpret_cast<uint4*>(k_out + to)[1] = k[1];
+  reinterpret_cast<uint4*>(v_out + to)[0] = v[0];
+  reinterpret_cast<uint4*>(v_out + to)[1] = v[1];
 }
 
 int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out) {
@@ -313,11 +333,11 @@ extern "C" int dq_kv4_read(const dq_kv4_batch* batch, void* k_out_bf16, void* v_
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   auto* k = static_cast<unsigned short*>(k_out_bf16);
   auto* v = static_cast<unsigned short*>(v_out_bf16);
-  const int lanes = 2 * c.hkv * batch->head_dim / 16;
-  const dim3 grid(c.T, (lanes + 127) / 128);
+  const int lanes = c.hkv * batch->head_dim / 16;
+  const dim3 grid(c.T, (lanes + 63) / 64);
   if (batch->head_dim == 128)
-    DQ_CHECK_CUDA(launch_pdl(kv4_read_kernel<128>, grid, dim3(128), 0, cs, c, k, v));
+    DQ_CHECK_CUDA(launch_pdl(kv4_read_kernel<128>, grid, dim3(64), 0, cs, c, k, v));
   else
-    DQ_CHECK_CUDA(launch_pdl(kv4_read_kernel<64>, grid, dim3(128), 0, cs, c, k, v));
+    DQ_CHECK_CUDA(launch_pdl(kv4_read_kernel<64>, grid, dim3(64), 0, cs, c, k, v));
   return DQ_OK;
 }
