@@ -369,6 +369,10 @@ class Decoder:
             raise ValueError("kv must be 'bf16' or 'int4'")
         if kv == "bf16" and (window or sinks):
             raise ValueError("a window and sinks need the paged cache (kv='int4')")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        if kv == "int4" and (self.cfg.head_dim not in (64, 128) or page_size not in (16, 32, 64, 128, 256)):
+            raise ValueError("the paged cache takes head_dim 64 or 128 and pages of 16, 32, 64, 128 or 256 tokens")
         self.max_len = max_len
         self.paged = None
         if kv == "int4":

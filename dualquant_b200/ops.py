@@ -679,7 +679,8 @@ def kv4_append(qkv: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tensor, 
     queries and keys behind the position rotation, which spreads outlier channels of keys over the 4-bit grid and leaves
     q . k as it is.  All index tensors are read on the device; rows from cu_new[B] on are left as they were.  A token without
     a place (negative position, behind the table row or the rotation tables) gets a zero query row and is not written, nor is
-    one whose page number lies outside of the cache."""
+    one whose page number lies outside of the cache.  No two tokens of a call may have the same slot of a page: either could
+    stay."""
     return _lib.host().kv4_append(qkv, cos_tab, sin_tab, cache, block_table, kv_len, hq, cu_new, bool(rotate))
 
 

@@ -158,3 +158,15 @@ def test_refusals():
         m.prefill(ids, pos0=-1)
     with pytest.raises(ValueError):
         make(1, head_dim=32, heads=16, kv_heads=4).alloc_cache(1, 32, kv="int4")
+
+
+def test_refused_caches_leave_the_one_that_is_there():
+    m = make(1)
+    ids = torch.arange(8, device=DEV)[None]
+    m.alloc_cache(1, 32, kv="int4", page_size=16)
+    want = m.prefill(ids)
+    for bad in (dict(kv="int4", page_size=0), dict(kv="int4", page_size=-16), dict(kv="int4", window=-1),
+                dict(kv="int4", window=4, sinks=-1)):
+        with pytest.raises(ValueError):
+            m.alloc_cache(1, 32, **bad)
+    assert torch.equal(m.prefill(ids), want)
