@@ -84,6 +84,30 @@ __device__ __forceinline__ int kv4_find(const Kv4Batch& c, int row, int lane, in
   return c.B;
 }
 
+// The same for the lanes of a warp that have N rows from `row` on, each its `mine`-th; rows behind the last are none.
+template <int N>
+__device__ __forceinline__ void kv4_find_rows(const Kv4Batch& c, int row, int lane, int mine, int* b, int* pos) {
+  if (c.cu_new == nullptr) {
+    const int n = c.T / c.B;
+    if (row + mine < c.T) {
+      *b = (row + mine) / n;
+      *pos = min(max(c.kv_len[*b], 0), kKv4Far) - n + (row + mine - *b * n);
+    }
+    return;
+  }
+  for (int base = 0; base < c.B; base += 32) {
+    Kv4Seq s = {0, 0, 0};
+    if (base + lane < c.B) s = kv4_seq(c, base + lane);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t has = __ballot_sync(0xFFFFFFFFu, row + i >= s.row0 && row + i - s.row0 < s.n);
+      const int l = (__ffs(has) - 1) & 31, p = __shfl_sync(0xFFFFFFFFu, s.kv - s.n + (row + i - s.row0), l);
+      if (has != 0 && i == mine && *b == c.B) *b = base + l, *pos = p;
+    }
+    if (__all_sync(0xFFFFFFFFu, *b < c.B)) break;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // Division of the work.  A segment is (sequence, key/value head, tile of query rows); its rows are (token, query head of
 // the group) pairs, token-major.  It reads the tokens that any of its rows sees, in tiles of TK tokens: with a window, first

@@ -595,3 +595,21 @@ def test_batches_of_more_sequences_than_lanes(B, new):
     out = ops.kv4_attention(q, ops.KV4Cache(pages, 64, 16), table, i32(lengths), cu_of(rows), new)
     want = ref.attention(q, ks, vs, rows, lengths)
     assert bool(((out.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths)).all())
+
+
+@pytest.mark.parametrize("hd,hkv", [(64, 3), (128, 1), (128, 5)])
+def test_read_of_warps_whose_rows_belong_to_several_sequences(hd, hkv):
+    gen = torch.Generator().manual_seed(hd + hkv)
+    rows = [1, 2, 0, 1, 5, 1, 0, 0, 3] * 8 + [37]
+    lengths = [n + (7 * i) % 30 if n else 0 for i, n in enumerate(rows)]
+    pages, table, ks, vs = ref.make_cache(gen, len(rows), lengths, hkv, hd, 16)
+    total = sum(rows)
+    for cu in (cu_of(rows), None):
+        if cu is None:
+            rows, lengths, ks, vs, table = [5] * 7, [37] * 7, ks[-1:] * 7, vs[-1:] * 7, table[-1:].repeat(7, 1)
+            total = 35
+        k, v = ops.kv4_read(ops.KV4Cache(pages, hd, 16), table, i32(lengths), total, cu)
+        for got, want in ((k, ks), (v, vs)):
+            want = torch.cat([w[:, m - n : m].transpose(0, 1) for w, n, m in zip(want, rows, lengths)])
+            # fp32 fma of an exact product (2^-24), then bf16
+            assert bool(((got.double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -23) + 1e-7).all())
