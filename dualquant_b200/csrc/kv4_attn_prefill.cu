@@ -29,6 +29,7 @@ namespace dq {
 
 constexpr int kPreThreads = 512;
 constexpr int kPreStages = 2;
+constexpr int kPreRaw = 3;        // keys or values of a converting warp's tiles that are on their way
 constexpr int kPreLoaders = 3;    // warps that bring the queries
 
 template <int HD>
@@ -40,7 +41,7 @@ struct PreSmem {
   static constexpr int kOffV = kOffK + kPreStages * kOperand;
   static constexpr int kRaw = 32 * (HD / 2 + 4);       // a converting warp's codes and pairs of 32 keys or values
   static constexpr int kOffRaw = kOffV + kPreStages * kOperand;
-  static constexpr int kOffBar = kOffRaw + 4 * 2 * kRaw;
+  static constexpr int kOffBar = kOffRaw + 4 * kPreRaw * kRaw;
   static constexpr int kBars = 6 + 4 * kPreStages + 10;
   static constexpr int kOffValid = kOffBar + kBars * 8;
   static constexpr int kOffMul = kOffValid + 4 * 4;            // [256] what a row's scores have to be multiplied with
@@ -517,10 +518,10 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       look_up();
     };
     // codes [32][HD / 2] and pairs [32] of the warp's tokens; pieces that are not there are left as they are in shared memory
-    uint8_t* const raw = smem + L::kOffRaw + w * 2 * L::kRaw;
-    auto copy = [&](bool values) {
+    uint8_t* const raw = smem + L::kOffRaw + w * kPreRaw * L::kRaw;
+    auto copy = [&](bool values, int place) {
       if (more) {
-        const uint32_t dst = smem_u32(raw) + (values ? L::kRaw : 0);
+        const uint32_t dst = smem_u32(raw) + place * L::kRaw;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if ((got >> i) & 1u) {
@@ -542,23 +543,26 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     uint32_t column[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) column[e] = ((((q & 1) << 2) + (e ^ turned)) ^ (in & 7)) << 4;
-    // keys of tile 0, values of tile 0, keys of tile 1 ...: one is converted while the next two are on the way
+    // keys of tile 0, values of tile 0, keys of tile 1 ...: one is converted while the next ones are on the way
+    static_assert(kPreRaw == 3, "keys of the next tile are asked for before this one is converted");
     look_up();
     seek();
-    copy(false);
-    copy(true);
+    copy(false, 0);
+    copy(true, 1);
     uint32_t got_now = got;
-    int left_now = left;
+    int left_now = left, place = 0;
+    seek();
+    copy(false, 2);
     bool values = false, last = false;
     for (uint32_t n = 0; ok && !last;) {
       const int stage = n % kPreStages;
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(kPreRaw - 1) : "memory");
       __syncwarp();
       ok = mbar_wait((values ? v_empty : k_empty) + stage, ((n / kPreStages) & 1) ^ 1, &s_abort, 45);
       // (slot n % 4 was last read for tile n - 4: the products of tile n - 2, which are done, waited for that)
       if (!values && lane == 0)
         reinterpret_cast<volatile uint8_t*>(smem + L::kOffValid)[(n & 3) * 4 + w] = static_cast<uint8_t>(got_now);
-      uint8_t* const from = raw + (values ? L::kRaw : 0);
+      uint8_t* const from = raw + place * L::kRaw;
       // tokens that are not there become zeros: their weights are zero, and zero times what a slot may hold is not
       if (left_now < 32 || got_now != 3u) {
         if (lane >= left_now || !((got_now >> (lane >> 4)) & 1u)) reinterpret_cast<uint32_t*>(from + 32 * (HD / 2))[lane] = 0;
@@ -580,14 +584,15 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       fence_proxy_async_smem();
       mbar_arrive((values ? v_full : k_full) + stage);
       __syncwarp();  // every lane has read the codes
-      if (!values) seek();  // the tile behind this one
-      copy(values);
-      if (values) {
+      if (values) {  // the tile behind this one is next, and the one behind that is asked for
         last = !more;
         got_now = got;
         left_now = left;
         ++n;
+        seek();
       }
+      copy(!values, place);
+      place = place == kPreRaw - 1 ? 0 : place + 1;
       values = !values;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");

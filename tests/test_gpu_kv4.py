@@ -613,3 +613,16 @@ def test_read_of_warps_whose_rows_belong_to_several_sequences(hd, hkv):
             want = torch.cat([w[:, m - n : m].transpose(0, 1) for w, n, m in zip(want, rows, lengths)])
             # fp32 fma of an exact product (2^-24), then bf16
             assert bool(((got.double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -23) + 1e-7).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [[3], [4], [2, 5, 0, 3], [9, 1]])
+def test_attention_of_more_than_one_tile_of_eight_rows(hd, new):
+    gen = torch.Generator().manual_seed(hd + len(new))
+    lengths = [n + 333 * (i + 1) for i, n in enumerate(new)]
+    pages, table, ks, vs = ref.make_cache(gen, len(new), lengths, 2, hd, 16)
+    q = torch.randn(sum(new), 16, hd, generator=gen).to(torch.bfloat16).cuda()
+    for most, window, sinks in ((max(new), 0, 0), (4, 0, 0), (4, 70, 5)):
+        out = ops.kv4_attention(q, ops.KV4Cache(pages, hd, 16), table, i32(lengths), cu_of(new), most, window=window, sinks=sinks)
+        want = ref.attention(q, ks, vs, new, lengths, window, sinks)
+        assert bool(((out.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths)).all())
