@@ -399,7 +399,7 @@ __host__ __device__ constexpr size_t kv4_partial_floats(int R, int hd) { return 
 
 // Tiles of the two attention kernels: tokens, query rows, and the least tiles of a CTA.
 constexpr int kDecTile = 32, kDecLeast = 4;                    // 8 or 16 rows
-constexpr int kPreTile = 128, kPreRows = 256, kPreLeast = 2;
+constexpr int kPreTile = 128, kPreLeast = 2;                 // 128 or 256
 constexpr float kKv4NoMax = -1e30f;  // reference point of a row that has seen no token
 
 int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out);
@@ -419,6 +419,6 @@ struct Kv4AttnArgs {
 
 int kv4_decode_resident(int hd, int R);  // CTAs per SM
 int launch_kv4_decode(const Kv4AttnArgs& a, int hd, int R, int grid, cudaStream_t s);
-int launch_kv4_prefill(const Kv4AttnArgs& a, int hd, int grid, cudaStream_t s, DeviceState* st);
+int launch_kv4_prefill(const Kv4AttnArgs& a, int hd, int R, int grid, cudaStream_t s, DeviceState* st);
 
 }  // namespace dq

@@ -108,7 +108,7 @@ kv4_combine_kernel(const __grid_constant__ Kv4AttnArgs a) {
   }
 }
 
-// How a call runs: R query rows a segment (8, 16: kv4_decode_kernel, 256: kv4_prefill_kernel) on `grid` CTAs.
+// How a call runs: R query rows a segment (8, 16: kv4_decode_kernel, 128, 256: kv4_prefill_kernel) on `grid` CTAs.
 struct Kv4Plan {
   int R, grid;
   size_t join_bytes, bytes;  // workspace
@@ -118,15 +118,17 @@ struct Kv4Plan {
 static Kv4Plan kv4_plan(const Kv4Batch& c, int G, int hd, int max_new, DeviceState* st) {
   Kv4Plan p;
   const int64_t rows = static_cast<int64_t>(G) * max_new;
-  // The few-rows kernel reads the cache once for every 16 rows, the other one takes up to 256 at the cost of one.  32 heads of
-  // 128 over 8, us, few / many: 16 rows over 16 x 4000 tokens 36 / 69, over 8 x 30000 83 / 215; 32 rows 58 / 70, 150 / 216 (and
-  // 20 / 16 over 1 x 4000); 48 rows 82 / 71, 219 / 217; 64 rows 100 / 72, 286 / 218.
-  p.R = rows <= 8 ? 8 : rows <= 32 ? 16 : kPreRows;
-  const int tile = p.R == kPreRows ? kPreTile : kDecTile, least = p.R == kPreRows ? kPreLeast : kDecLeast;
+  // The few-rows kernel reads the cache once for every 16 rows, the other one once for up to 128 or 256.  32 heads of 128 over 8,
+  // us: 16, 32, 48, 64 rows over 16 x 4000 tokens 36, 58, 82, 100 in tiles of 16, and 61 to 62 for 48 and 64 in one of 128; over
+  // 8 x 30000 tokens 83, 150, 219, 286 and 184 to 185; over 1 x 4000 14, 20, 22, 23 and 16 to 17.  A row tile of 128 by itself
+  // in the two-tile kernel: 72, 218 and 17.
+  p.R = rows <= 8 ? 8 : rows <= 32 ? 16 : rows <= 128 ? 128 : 256;
+  const bool many = p.R >= 128;
+  const int tile = many ? kPreTile : kDecTile, least = many ? kPreLeast : kDecLeast;
   const int64_t row_tiles = (static_cast<int64_t>(c.T) * G + p.R - 1) / p.R + c.B;
   const int64_t units = row_tiles * c.hkv * ((c.capacity + tile - 1) / tile + 1);
   const int64_t most = (units + least - 1) / least;
-  const int64_t fill = st->sm_count * (p.R == kPreRows ? 1 : kv4_decode_resident(hd, p.R));
+  const int64_t fill = st->sm_count * (many ? 1 : kv4_decode_resident(hd, p.R));
   p.grid = units >= (1ll << 31) ? 0 : static_cast<int>(most < fill ? most : fill);
   p.join_bytes = (static_cast<size_t>(p.grid) * sizeof(Kv4Join) + 255) / 256 * 256;
   p.bytes = p.join_bytes + static_cast<size_t>(p.grid) * 2 * kv4_partial_floats(p.R, hd) * 4;
@@ -138,6 +140,16 @@ static int launch_combine(const Kv4AttnArgs& a, int grid, cudaStream_t s) {
   constexpr int y = WARPS > 1 ? 4 : 8;
   DQ_CHECK_CUDA(launch_pdl(kv4_combine_kernel<HD, R, WARPS>, dim3(grid, y), dim3(256), 0, s, a));
   return DQ_OK;
+}
+
+template <int HD>
+static int launch_combine_of(const Kv4AttnArgs& a, const Kv4Plan& p, cudaStream_t s) {
+  switch (p.R) {
+    case 8: return launch_combine<HD, 8, 8>(a, p.grid, s);
+    case 16: return launch_combine<HD, 16, 8>(a, p.grid, s);
+    case 128: return launch_combine<HD, 128, 1>(a, p.grid, s);
+    default: return launch_combine<HD, 256, 1>(a, p.grid, s);
+  }
 }
 
 }  // namespace dq
@@ -186,11 +198,7 @@ extern "C" int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, i
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.join_bytes);
   a.scale2 = scale * 1.4426950408889634f;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  rc = p.R == kPreRows ? launch_kv4_prefill(a, hd, p.grid, cs, st) : launch_kv4_decode(a, hd, p.R, p.grid, cs);
+  rc = p.R >= 128 ? launch_kv4_prefill(a, hd, p.R, p.grid, cs, st) : launch_kv4_decode(a, hd, p.R, p.grid, cs);
   if (rc != DQ_OK || p.grid == 1) return rc;
-  if (hd == 128)
-    return p.R == 8 ? launch_combine<128, 8, 8>(a, p.grid, cs) : p.R == 16 ? launch_combine<128, 16, 8>(a, p.grid, cs)
-                                                                            : launch_combine<128, kPreRows, 1>(a, p.grid, cs);
-  return p.R == 8 ? launch_combine<64, 8, 8>(a, p.grid, cs) : p.R == 16 ? launch_combine<64, 16, 8>(a, p.grid, cs)
-                                                                         : launch_combine<64, kPreRows, 1>(a, p.grid, cs);
+  return hd == 128 ? launch_combine_of<128>(a, p, cs) : launch_combine_of<64>(a, p, cs);
 }

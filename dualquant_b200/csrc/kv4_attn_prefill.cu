@@ -1,7 +1,7 @@
 // Attention of many query rows per sequence over the paged 4-bit cache (prompts, pieces of prompts) on tcgen05.
 //
 // A segment has up to 256 query rows, (token, query head) pairs of one key/value head: two tiles of 128 rows against the same
-// keys and values, tiles of 128 tokens.  One persistent CTA per SM, sixteen warps:
+// keys and values, tiles of 128 tokens (ROWS = 128: one row tile, whose warps 4-7 do nothing).  One persistent CTA per SM, sixteen warps:
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: scores out of tensor memory, the running maximum and sum,
 //                    weights back to tensor memory, at the end the output
 //   warps 8-11       codes from the pages to fp16 keys and values (fma(c, scale, zero), one rounding) in shared memory
@@ -45,7 +45,7 @@ struct PreSmem {
   static constexpr int kBars = 6 + 4 * kPreStages + 10;
   static constexpr int kOffValid = kOffBar + kBars * 8;
   static constexpr int kOffMul = kOffValid + 4 * 4;            // [256] what a row's scores have to be multiplied with
-  static constexpr int kOffCursor = kOffMul + kPreRows * 4;
+  static constexpr int kOffCursor = kOffMul + 256 * 4;
   static constexpr int kOffTmem = kOffCursor + static_cast<int>((sizeof(Kv4Cursor) + 8 + 15) / 16 * 16);
   static constexpr int kBytes = kOffTmem + 16 + 1024;  // (the operands start at a multiple of 1024)
 };
@@ -133,11 +133,12 @@ __device__ __forceinline__ int pre_groups(const Kv4Batch& c, const Kv4Cursor& k)
   return k.u1 == k.span.count && hi <= k.span.tile(k.u1 - 1) * kPreTile + 64 ? n - 1 : n;
 }
 
-template <int HD>
+template <int HD, int ROWS>
 __global__ void __launch_bounds__(kPreThreads, 1)
 kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   grid_dep_launch_dependents();
   using L = PreSmem<HD>;
+  constexpr bool kOne = ROWS == 128;  // segments of one row tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ volatile int s_abort;
@@ -185,7 +186,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   }
   grid_dep_wait();
   if (warp == 0) {
-    const Kv4Start k = kv4_begin_any<kPreTile>(a.c, a.m, a.g, kPreRows, kPreLeast, a.grid, lane);
+    const Kv4Start k = kv4_begin_any<kPreTile>(a.c, a.m, a.g, ROWS, kPreLeast, a.grid, lane);
     if (lane == 0) {
       if (k.any) found = k.k;
       else a.join[blockIdx.x].parts = 0;
@@ -222,7 +223,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     // groups of the next.  (First round: no output.)
     for (;;) {
       float mul_next = 1.0f;
-      if (more && ok && (tile == 0 || next.seq.n * a.g.G - next.rt * kPreRows > 128)) {
+      if (more && ok && (tile == 0 || (!kOne && next.seq.n * a.g.G - next.rt * ROWS > 128))) {
         // A row as fp16 times a power of two that brings its largest element to [2^14, 2^15): HD / 16 lanes a row, in place
         constexpr int kRowLanes = HD / 16, kRowsAtOnce = 32 / kRowLanes;
         const int l = lane % kRowLanes;
@@ -277,9 +278,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         mul_next = mul_out[row_in];
       }
       if (!fresh) {
-        const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
-        if (tile == 0 || rows > 128) {
-          const int r = at.rt * kPreRows + tile * 128 + row_in;
+        const int rows = at.seq.n * a.g.G - at.rt * ROWS;
+        if (tile == 0 || (!kOne && rows > 128)) {
+          const int r = at.rt * ROWS + tile * 128 + row_in;
           const bool there = tile * 128 + row_in < rows;
           const int i_tok = there ? a.g.by(r) : 0, head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
           const int64_t out_at = (static_cast<int64_t>(at.seq.row0 + i_tok) * a.c.hkv * a.g.G + head) * HD;
@@ -292,8 +293,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
           float by = whole_segment ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
           if (!finite && l != 0.0f) by = __int_as_float(0x7FC00000);
-          float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(kPreRows, HD);
-          float* part_o = part + 2 * kPreRows + (tile * 128 + row_in) * HD;
+          float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (is_first ? 0 : 1)) * kv4_partial_floats(ROWS, HD);
+          float* part_o = part + 2 * ROWS + (tile * 128 + row_in) * HD;
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             uint32_t o[32];
@@ -354,8 +355,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           Kv4Join j;
           j.parts = 1 + (at.span.count - at.u1 + share - 1) / share;
           j.slot = is_first ? 0 : 1;
-          j.rows = min(rows, kPreRows);
-          j.first_row = at.rt * kPreRows;
+          j.rows = min(rows, ROWS);
+          j.first_row = at.rt * ROWS;
           j.row0 = at.seq.row0;
           j.h = at.h;
           a.join[blockIdx.x] = j;
@@ -366,11 +367,11 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       if (!more || !ok) break;
       at = next;
       fresh = false;
-      const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
-      if (tile == 0 || rows > 128) {
+      const int rows = at.seq.n * a.g.G - at.rt * ROWS;
+      if (tile == 0 || (!kOne && rows > 128)) {
         const int n_groups = pre_groups(a.c, at);
         const bool there = tile * 128 + row_in < rows;
-        const int i_tok = there ? a.g.by(at.rt * kPreRows + tile * 128 + row_in) : 0;
+        const int i_tok = there ? a.g.by(at.rt * ROWS + tile * 128 + row_in) : 0;
         const int kv = min(at.seq.kv, a.c.capacity);
         const int p_row = at.seq.kv - at.seq.n + i_tok;
         const int hi = there ? min(p_row + 1, kv) : 0;                   // tokens lo ... hi - 1 and those below `first`
@@ -386,7 +387,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         for (int j = 0; j < n_groups && ok; ++j) {
           const int tok = at.span.tile(at.u0 + (j >> 1)) * kPreTile + 64 * (j & 1);
           const int half = j & 1;
-          const uint32_t t_b = t_s + 64 * half;
+          const uint32_t t_b = t_s + ((kOne ? (j << 6) & 128 : 0) | (half << 6));
           if (half == 0) {
             ok = mbar_wait(s_full + tile, count[0]++ & 1, &s_abort, 42);
             tc_fence_after();
@@ -423,8 +424,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             m = to;
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
-              // the groups before are in O: those of earlier tiles are since there are scores of this one
+              // the groups before are in O: of two row tiles those of earlier tiles are since there are scores of this one
               if (half == 1) ok = ok && mbar_wait(o_done + 2 * tile, (count[0] - 1) & 1, &s_abort, 43);
+              else if (kOne) ok = ok && mbar_wait(o_done + 1, (count[1] - 1) & 1, &s_abort, 46);
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -467,7 +469,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           mbar_arrive(p_full + 2 * tile + half);
         }
       }
-      more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, next);
+      more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, ROWS, next);
     }
     if (threadIdx.x == 0 && !goes_on) a.join[blockIdx.x].parts = 0;
   } else if (warp < 12) {
@@ -487,7 +489,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     int slot[2], left = 0;
     auto look_up = [&]() {
       while (coming && u >= at.u1) {
-        coming = kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at);
+        coming = kv4_next_segment<kPreTile>(a.c, a.m, a.g, ROWS, at);
         u = at.u0;
       }
       if (!coming) return;
@@ -570,16 +572,27 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       }
       const uint8_t *src = from + in * (HD / 2) + q * 16, *pairs = from + 32 * (HD / 2) + in * 4;
       uint8_t* const to = smem + (values ? L::kOffV : L::kOffK) + stage * L::kOperand + to_lane;
+      // Beside one row tile these warps are what a tile waits for, and all loads come first, which the compiler cannot move over
+      // stores; beside two row tiles that took their softmax's issue slots (409 to 411 us).
+      constexpr int kAtOnce = kOne ? kLoads : 1;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const uint2 c01 = *reinterpret_cast<const uint2*>(src + i * kStep * (HD / 2) + 4 * turned);
-        const uint2 c23 = *reinterpret_cast<const uint2*>(src + i * kStep * (HD / 2) + (8 - 4 * turned));
-        const __half2 pair = *reinterpret_cast<const __half2*>(pairs + i * kStep * 4);
-        const __half2 sc = __low2half2(pair), ze = __high2half2(pair);
-        const uint32_t c[4] = {c01.x, c01.y, c23.x, c23.y};
+      for (int i0 = 0; i0 < kLoads; i0 += kAtOnce) {
+        uint2 c01[kAtOnce], c23[kAtOnce];
+        __half2 pair[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint4*>(to + column[e] + i * kStep * 128) = pre_expand(c[e], sc, ze);
+        for (int i = 0; i < kAtOnce; ++i) {
+          c01[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * kStep * (HD / 2) + 4 * turned);
+          c23[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * kStep * (HD / 2) + (8 - 4 * turned));
+          pair[i] = *reinterpret_cast<const __half2*>(pairs + (i0 + i) * kStep * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const __half2 sc = __low2half2(pair[i]), ze = __high2half2(pair[i]);
+          const uint32_t c[4] = {c01[i].x, c01[i].y, c23[i].x, c23[i].y};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(to + column[e] + (i0 + i) * kStep * 128) = pre_expand(c[e], sc, ze);
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive((values ? v_full : k_full) + stage);
@@ -601,65 +614,78 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     if (elect_one()) {
       constexpr uint32_t kIdescS = pre_idesc(128, 128, false), kIdescO = pre_idesc(128, HD, true);
       uint32_t q_phase[2] = {0, 0}, p_phase[2][2] = {{0, 0}, {0, 0}}, n = 0;  // n: token tiles so far
-      auto scores = [&](int t, uint32_t tile_number, bool last) {
+      auto scores = [&](int t, int at_s, uint32_t tile_number, bool last) {
         const uint32_t qa = base + L::kOffQ + t * L::kOperand, ka = base + L::kOffK + tile_number % kPreStages * L::kOperand;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          pre_mma_ss(tmem + t * 128, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
+          pre_mma_ss(tmem + at_s * 128, umma_desc_k_sw128(qa + (k >> 2) * L::kHalf + (k & 3) * 32),
                      umma_desc_k_sw128(ka + (k >> 2) * L::kHalf + (k & 3) * 32), kIdescS, k > 0);
         umma_commit(s_full + t);
         if (last) umma_commit(q_empty + t);
       };
-      auto values = [&](int t, uint32_t tile_number, int half, bool add) {
+      auto values = [&](int t, int at_s, uint32_t tile_number, int half, bool add) {
         const uint32_t va = base + L::kOffV + tile_number % kPreStages * L::kOperand + half * 8192;
         ok = ok && mbar_wait(p_full + 2 * t + half, p_phase[t][half]++ & 1, &s_abort, 51);
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          pre_mma_ts(tmem + 256 + t * HD, tmem + t * 128 + half * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf), kIdescO,
+          pre_mma_ts(tmem + 256 + t * HD, tmem + at_s * 128 + half * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf), kIdescO,
                      add || k > 0);
         umma_commit(o_done + 2 * t + half);
       };
-      // A row tile's next scores follow its weights' second half: products run in order, so those weights have been read.
+      // Of two row tiles, a tile's next scores follow its weights' second half: products run in order, so those weights have been
+      // read.  A row tile by itself has the other's scores' columns for every second token tile; its next scores follow its
+      // weights' first half, whose arrival says that every row has begun with the scores before.
       for (;;) {
-        const int rows = at.seq.n * a.g.G - at.rt * kPreRows, groups = pre_groups(a.c, at), tiles = (groups + 1) / 2;
-        const bool two = rows > 128;
+        const int rows = at.seq.n * a.g.G - at.rt * ROWS, groups = pre_groups(a.c, at), tiles = (groups + 1) / 2;
+        const bool two = !kOne && rows > 128;
         ok = ok && mbar_wait(k_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 49);
         ok = ok && mbar_wait(q_full, q_phase[0]++ & 1, &s_abort, 47);
         if (!ok) break;
         tc_fence_after();
-        scores(0, n, tiles == 1);
+        scores(0, 0, n, tiles == 1);
         if (two) {
           ok = mbar_wait(q_full + 1, q_phase[1]++ & 1, &s_abort, 48);
           if (!ok) break;
           tc_fence_after();
-          scores(1, n, tiles == 1);
+          scores(1, 1, n, tiles == 1);
         }
         umma_commit(k_empty + n % kPreStages);
 #pragma unroll 1
         for (int j = 0; j < tiles && ok; ++j, ++n) {
           const bool more = j + 1 < tiles, both = 2 * j + 1 < groups;
           ok = mbar_wait(v_full + n % kPreStages, (n / kPreStages) & 1, &s_abort, 50);
-          values(0, n, 0, j > 0);
-          if (both) values(0, n, 1, true);
-          if (more) {
-            ok = ok && mbar_wait(k_full + (n + 1) % kPreStages, ((n + 1) / kPreStages) & 1, &s_abort, 52);
-            if (!ok) break;
-            tc_fence_after();
-            scores(0, n + 1, j + 2 == tiles);
-          }
-          if (two) {
-            values(1, n, 0, j > 0);
-            if (both) values(1, n, 1, true);
-            if (!ok) break;
-            if (more) scores(1, n + 1, j + 2 == tiles);
+          if constexpr (!kOne) {
+            values(0, 0, n, 0, j > 0);
+            if (both) values(0, 0, n, 1, true);
+            if (more) {
+              ok = ok && mbar_wait(k_full + (n + 1) % kPreStages, ((n + 1) / kPreStages) & 1, &s_abort, 52);
+              if (!ok) break;
+              tc_fence_after();
+              scores(0, 0, n + 1, j + 2 == tiles);
+            }
+            if (two) {
+              values(1, 1, n, 0, j > 0);
+              if (both) values(1, 1, n, 1, true);
+              if (!ok) break;
+              if (more) scores(1, 1, n + 1, j + 2 == tiles);
+            }
+          } else {
+            values(0, j & 1, n, 0, j > 0);
+            if (more) {
+              ok = ok && mbar_wait(k_full + (n + 1) % kPreStages, ((n + 1) / kPreStages) & 1, &s_abort, 53);
+              if (!ok) break;
+              tc_fence_after();
+              scores(0, (j & 1) ^ 1, n + 1, j + 2 == tiles);
+            }
+            if (both) values(0, j & 1, n, 1, true);
           }
           if (!ok) break;
           umma_commit(v_empty + n % kPreStages);
           if (more) umma_commit(k_empty + (n + 1) % kPreStages);
         }
-        if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
+        if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, ROWS, at)) break;
       }
     }
     __syncwarp();
@@ -670,9 +696,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const int w = warp - 13, l = lane % kRowLanes, row0 = w * kRowsAtOnce + lane / kRowLanes;
     uint32_t uses[2] = {0, 0};
     for (;;) {
-      const int rows = at.seq.n * a.g.G - at.rt * kPreRows;
+      const int rows = at.seq.n * a.g.G - at.rt * ROWS;
 #pragma unroll 1
-      for (int tile = 0; tile < (rows > 128 ? 2 : 1); ++tile) {
+      for (int tile = 0; tile < (!kOne && rows > 128 ? 2 : 1); ++tile) {
         const uint32_t use = uses[tile]++;
         ok = ok && mbar_wait(q_empty + tile, (use & 1) ^ 1, &s_abort, 55);
         // 16-byte columns 2l and 2l + 1 of a row
@@ -681,7 +707,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
 #pragma unroll 1
         for (int row = row0; row < 128; row += kStep) {
           const bool there = tile * 128 + row < rows;
-          const int r = at.rt * kPreRows + tile * 128 + row, i_tok = there ? a.g.by(r) : 0;
+          const int r = at.rt * ROWS + tile * 128 + row, i_tok = there ? a.g.by(r) : 0;
           const int head = at.h * a.g.G + (there ? r - i_tok * a.g.G : 0);
           const unsigned short* src =
               a.q + static_cast<int64_t>(at.seq.row0 + i_tok) * a.q_row + static_cast<int64_t>(head) * a.q_head + 16 * l;
@@ -691,7 +717,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         mbar_arrive(q_raw + tile);
       }
-      if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, kPreRows, at)) break;
+      if (!ok || !kv4_next_segment<kPreTile>(a.c, a.m, a.g, ROWS, at)) break;
     }
   }
   // every product has been waited for by the softmax of its row tile (or a wait ran out)
@@ -702,21 +728,26 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   if (threadIdx.x == 0 && s_abort != 0) atomicExch(status, s_abort);
 }
 
-template <int HD>
+template <int HD, int ROWS>
 static int init_prefill() {
-  DQ_CHECK_CUDA(cudaFuncSetAttribute(kv4_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, PreSmem<HD>::kBytes));
+  DQ_CHECK_CUDA(cudaFuncSetAttribute(kv4_prefill_kernel<HD, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PreSmem<HD>::kBytes));
   return DQ_OK;
 }
 int init_kv4_prefill_kernels() {
-  const int rc = init_prefill<64>();
-  return rc == DQ_OK ? init_prefill<128>() : rc;
+  int rc = init_prefill<64, 128>();
+  if (rc == DQ_OK) rc = init_prefill<64, 256>();
+  if (rc == DQ_OK) rc = init_prefill<128, 128>();
+  if (rc == DQ_OK) rc = init_prefill<128, 256>();
+  return rc;
 }
-int launch_kv4_prefill(const Kv4AttnArgs& a, int hd, int grid, cudaStream_t s, DeviceState* st) {
-  if (hd == 128)
-    DQ_CHECK_CUDA(launch_pdl(kv4_prefill_kernel<128>, dim3(grid), dim3(kPreThreads), PreSmem<128>::kBytes, s, a, st->status_dev));
-  else
-    DQ_CHECK_CUDA(launch_pdl(kv4_prefill_kernel<64>, dim3(grid), dim3(kPreThreads), PreSmem<64>::kBytes, s, a, st->status_dev));
+template <int HD, int ROWS>
+static int launch_prefill(const Kv4AttnArgs& a, int grid, cudaStream_t s, DeviceState* st) {
+  DQ_CHECK_CUDA(launch_pdl(kv4_prefill_kernel<HD, ROWS>, dim3(grid), dim3(kPreThreads), PreSmem<HD>::kBytes, s, a, st->status_dev));
   return DQ_OK;
+}
+int launch_kv4_prefill(const Kv4AttnArgs& a, int hd, int R, int grid, cudaStream_t s, DeviceState* st) {
+  if (hd == 128) return R == 128 ? launch_prefill<128, 128>(a, grid, s, st) : launch_prefill<128, 256>(a, grid, s, st);
+  return R == 128 ? launch_prefill<64, 128>(a, grid, s, st) : launch_prefill<64, 256>(a, grid, s, st);
 }
 
 }  // namespace dq

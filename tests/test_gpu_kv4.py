@@ -626,3 +626,20 @@ def test_attention_of_more_than_one_tile_of_eight_rows(hd, new):
         out = ops.kv4_attention(q, ops.KV4Cache(pages, hd, 16), table, i32(lengths), cu_of(new), most, window=window, sinks=sinks)
         want = ref.attention(q, ks, vs, new, lengths, window, sinks)
         assert bool(((out.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths)).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("most,new", [(20, [20, 1, 11]), (32, [32]), (9, [9, 0, 4]), (32, [100, 32, 70]), (10, [200])])
+def test_attention_of_a_single_tile_of_128_rows(hd, most, new):
+    # 33 to 128 rows by the hint; tokens behind the last group of 64, rescaled rows and missing hints among them
+    gen = torch.Generator().manual_seed(hd + most)
+    lengths = [n + 100 * i + 613 for i, n in enumerate(new)]
+    pages, table, ks, vs = ref.make_cache(gen, len(new), lengths, 2, hd, 32)
+    q = (torch.randn(sum(new), 8, hd, generator=gen) * 3).to(torch.bfloat16).cuda()
+    for window, sinks in ((0, 0), (150, 3)):
+        out = ops.kv4_attention(q, ops.KV4Cache(pages, hd, 32), table, i32(lengths), cu_of(new), most, window=window, sinks=sinks)
+        want = ref.attention(q, ks, vs, new, lengths, window, sinks)
+        # keys are rounded to fp16: 2^-11 of each product's size in a score (|q| |k| / sqrt(d), four standard deviations: 4 * 3 * 3
+        # * 2^-11), which moves a weight by that much relative to the values' span
+        span = max(float((v.amax(-1) - v.amin(-1)).max()) for v in vs)
+        assert bool(((out.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths) + span * 36 * 2.0 ** -11).all())
