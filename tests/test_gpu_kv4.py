@@ -554,7 +554,8 @@ def test_calls_back_to_back_on_one_and_on_two_streams_give_the_same_bits():
     gen = torch.Generator().manual_seed(11)
     batches = []
     for new, lengths, heads in (([300, 0, 17, 128], [1700, 0, 900, 128], (8, 2, 128)), ([1] * 40, list(range(1, 4001, 100)), (8, 1, 64)),
-                                ([4, 2, 9], [3000, 77, 2000], (4, 4, 128)), ([700], [700], (4, 1, 64))):
+                                ([4, 2, 9], [3000, 77, 2000], (4, 4, 128)), ([700], [700], (4, 1, 64)),
+                                ([20, 9, 31], [3000, 500, 2000], (8, 2, 128)), ([100] * 5, [100, 2000, 900, 5000, 300], (2, 2, 64))):
         hq, hkv, hd = heads
         pages, table, _, _ = ref.make_cache(gen, len(new), lengths, hkv, hd, 32)
         q = torch.randn(sum(new), hq, hd, generator=gen).to(torch.bfloat16).cuda()
@@ -568,6 +569,7 @@ def test_calls_back_to_back_on_one_and_on_two_streams_give_the_same_bits():
         with torch.cuda.stream(streams[(i // 3) % 2 if i >= 100 else 0]):
             got.append((ops.kv4_attention(*args), want))
     torch.cuda.synchronize()
+    _lib.device_status(0)  # (no wait of a kernel has run out)
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in got)
 
 
