@@ -466,6 +466,11 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           }
           tmem_st_wait();
           tc_fence_before();
+          // Of a row tile by itself, scores of the next token tile follow the first half's weights: a warp may be here again while
+          // another has yet to bring its second half of the tile before, whose arrivals are counted, not named.  So nobody brings a
+          // second half before the last one's products are done (they are, but for a warp that was held up); that also keeps the
+          // phases that are waited for above and behind the segment one apart.
+          if (kOne && half == 1 && j > 1) ok = ok && mbar_wait(o_done + 1, (count[1] - 2) & 1, &s_abort, 57);
           mbar_arrive(p_full + 2 * tile + half);
         }
       }
@@ -636,7 +641,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       };
       // Of two row tiles, a tile's next scores follow its weights' second half: products run in order, so those weights have been
       // read.  A row tile by itself has the other's scores' columns for every second token tile; its next scores follow its
-      // weights' first half, whose arrival says that every row has begun with the scores before.
+      // weights' first half, whose arrival says that every row is through with the tile before, whose columns they take.
       for (;;) {
         const int rows = at.seq.n * a.g.G - at.rt * ROWS, groups = pre_groups(a.c, at), tiles = (groups + 1) / 2;
         const bool two = !kOne && rows > 128;
