@@ -402,6 +402,39 @@ constexpr int kDecTile = 32, kDecLeast = 4;                    // 8 or 16 rows
 constexpr int kPreTile = 128, kPreLeast = 2;                 // 128 or 256
 constexpr float kKv4NoMax = -1e30f;  // reference point of a row that has seen no token
 
+// A query row as fp16: times +-2^p, which brings its largest element to [2^14, 2^15) and gives it the scale's sign (0: a scale of
+// zero); scores of such elements are to be multiplied with `back`, which is positive.
+// Where the largest element times the scale would pass 2^64, `back` is taken of 2^64: scores stay finite and above kKv4NoMax, and
+// the row's weights are what they would be, one at the largest score and zero elsewhere (of scores of 2^64 keys fp32 resolves
+// 2^40 keys, and a key's smallest step is 2^-24).
+struct Kv4RowScale {
+  float up, back;
+};
+// big: bits of the row's largest bf16 element, 0 for a row that is not finite
+__device__ __forceinline__ Kv4RowScale kv4_row_scale(uint32_t big, float scale2) {
+  const int e = big > 0 ? static_cast<int>(big >> 7) - 127 : 0;
+  const int p = min(14 - e, 126);  // -113 ... 126
+  const int over = max(e + static_cast<int>((__float_as_uint(scale2) >> 23) & 255u) - 127 - 63, 0);
+  // (over > 0 only where e > -64: p + over lies in [-113, 126] or, with over, up to 78)
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + p) << 23);
+  const float back = fabsf(scale2) * __uint_as_float(static_cast<uint32_t>(127 - p - over) << 23);
+  return {scale2 > 0.0f ? up : scale2 < 0.0f ? -up : 0.0f, scale2 != 0.0f ? fmaxf(back, 1.2e-38f) : 1.0f};
+}
+
+// Weights are 2^(s mul - m) with one fused operation, whose product is not rounded as m once was: from |m| = 2^27 on they could
+// pass what fp16 holds, or all be zero.  From 2^24 on a row goes on in units 2^k of scores that keep |m| below that (m and mul divided by
+// it, `unit` multiplied: m * unit is the score).  Scores that such units bring together differ by less than 2^-19 of their size,
+// which a sum of 128 products in fp32 may not tell apart either.
+__device__ __forceinline__ void kv4_units(float& m, float& mul, float& unit) {
+  if (fabsf(m) >= 16777216.0f && m != kKv4NoMax) {
+    const uint32_t e = (__float_as_uint(m) >> 23) & 255u;  // 151 ... 215
+    const float by = __uint_as_float((277u - e) << 23);
+    m *= by;
+    mul *= by;
+    unit *= __uint_as_float((e - 23u) << 23);
+  }
+}
+
 int kv4_batch_of(const dq_kv4_batch* in, Kv4Batch* out);
 
 struct Kv4AttnArgs {

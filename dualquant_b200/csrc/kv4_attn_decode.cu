@@ -5,7 +5,7 @@
 //   q . (s c + z) = s (q . c) + z (q . 1),   sum_j p_j (s_j c_j + z_j) = sum_j (p_j s_j) c_j + sum_j p_j z_j
 // so that the products run on the bare codes.  A 4-bit code in the low bits of an fp16 word IS an fp16 number, the subnormal
 // c * 2^-24 (in bits 4 to 7: c * 2^-20): an AND makes two operands of mma.sync.m16n8k16, with no conversion, and the powers
-// of two go into the scores' scale, into every other query element, and into the last factor of the output.  A code costs
+// of two go into the row's factor, into every other query element, and into the last factor of the output.  A code costs
 // 0.6 (keys) and 0.75 (values) instructions.
 //
 // Both products are taken transposed, keys or head elements along the 16 rows and up to eight query rows along the columns
@@ -20,7 +20,8 @@
 //   * p_j s_j is fp16 (an mma operand, 2^-11 relative, in the row's own scale): the reference point m is taken of
 //     x_j + exponent(s_j), so that p_j s_j stays below 2^9 and what counts stays normal whatever the scales are;
 //   * m moves only where a row would pass 2^8 above it; l, sum p z and O are fp32.
-// Query rows are fp16 times a power of two of the tile: exact where a row is within 2^13 of the tile's largest value.
+// Query rows are fp16 times a power of two of the row: an element is exact down to 2^-27 of the row's largest one (fp16 has its
+// 8 bits down to 2^-17, every other element is taken times 1 / 16), and no row knows of its neighbours.
 //
 // 64 sequences of up to 16384 tokens, 8 heads of 128, four rows each: 1.14 GB in 219 us, 5.2 TB/s, 81 % of what a plain copy
 // moves.  The integer pipe is nearest to its end there (59 % of its cycles, issue slots 55 %): ANDs and shifts that take the
@@ -91,72 +92,63 @@ template <int HD, int NT>
 struct DecQuery {
   static constexpr int KS = HD / 16;  // steps of 16 head elements
   uint32_t f[NT][KS][2];
-  float2 zq[NT];     // sum of a row's elements, times scale log2(e); NaN for a row that is not finite
+  // of query rows 2t and 2t + 1:
+  float2 mul[NT];    // what s S' + z zq has to be multiplied with to be scores in base 2; positive
+  float2 zq[NT];     // sum of a row's elements, in units of S'; NaN for a row that is not finite
   int pos[NT][2];    // the row's position; -1: no such row
-  float mul;         // what S' has to be multiplied with to be scores in base 2
 
   // rows: the segment's query rows in shared memory, bf16, kQPitch bytes apart; rows that do not exist are zero
   __device__ __forceinline__ void load(const Kv4AttnArgs& a, const Kv4Cursor& k, const uint8_t* q_rows, int lane) {
     constexpr int R = 8 * NT, W = HD / 32;  // W: 32-bit words of codes per lane
     const int g = lane >> 2, t = lane & 3, rows = k.seq.n * a.g.G;
-    uint32_t raw[NT][W * 4];  // pairs of bf16
-    uint32_t top = 0;         // largest size of an element, as bf16 bits
-    float sum[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint8_t* src = q_rows + (nt * 8 + g) * kQPitch<HD> + t * (W * 16);
-      uint32_t big = 0;
-      float2 s[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      uint32_t raw[W * 4];  // pairs of bf16
+      uint32_t big = 0;     // largest size of an element, as bf16 bits
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * w);
         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          raw[nt][4 * w + j] = u[j];
+          raw[4 * w + j] = u[j];
           big = __vmaxu2(big, u[j] & 0x7FFF7FFFu);
-          s[j & 1] = __fadd2_rn(s[j & 1], make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u)));
         }
       }
-      s[0] = __fadd2_rn(s[0], s[1]);
-      float total = s[0].x + s[0].y;
       big = max(big & 0xFFFFu, big >> 16);
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
-        big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
-      }
+      for (int d = 1; d < 4; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
       const bool fine = big < 0x7F80u;  // no infinity and no NaN in the row
-      sum[nt] = fine ? total * a.scale2 : __int_as_float(0x7FC00000);
-      if (fine) {
-        top = max(top, big);
-      } else {
+      if (!fine) {
 #pragma unroll
-        for (int j = 0; j < W * 4; ++j) raw[nt][j] = 0;
+        for (int j = 0; j < W * 4; ++j) raw[j] = 0;
       }
-    }
+      const Kv4RowScale by = kv4_row_scale(fine ? big : 0, a.scale2);
+      float2 s[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    const int e = top > 0 ? static_cast<int>(top >> 7) - 127 : 0;
-    const int up = max(min(14 - e, 100), -103);  // largest element into [2^14, 2^15)
-    const float by = __int_as_float((up + 127) << 23);
-    mul = a.scale2 * __int_as_float((127 + 24 - up) << 23);
+      for (int j = 0; j < W * 4; ++j)
+        s[j & 1] = __ffma2_rn(make_float2(__uint_as_float(raw[j] << 16), __uint_as_float(raw[j] & 0xFFFF0000u)), both(by.up), s[j & 1]);
+      s[0] = __fadd2_rn(s[0], s[1]);
+      float total = s[0].x + s[0].y;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+      for (int d = 1; d < 4; d <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+      const float sum = fine ? total * 0x1p-24f : __int_as_float(0x7FC00000), back = by.back * 16777216.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           // elements 2u, 2u + 1 and 2u + 4, 2u + 5 of eight: the order of the nibbles (0, 4), (1, 5) ... of a word
-          const uint32_t p = raw[nt][4 * w + u], r = raw[nt][4 * w + u + 2];
-          const float2 even = __fmul2_rn(make_float2(__uint_as_float(p << 16), __uint_as_float(r << 16)), both(by));
+          const uint32_t p = raw[4 * w + u], r = raw[4 * w + u + 2];
+          const float2 even = __fmul2_rn(make_float2(__uint_as_float(p << 16), __uint_as_float(r << 16)), both(by.up));
           const float2 odd = __fmul2_rn(make_float2(__uint_as_float(p & 0xFFFF0000u), __uint_as_float(r & 0xFFFF0000u)),
-                                        both(by * 0.0625f));
+                                        both(by.up * 0.0625f));
           f[nt][2 * w + u][0] = half2_bits(even.x, even.y);
           f[nt][2 * w + u][1] = half2_bits(odd.x, odd.y);
         }
       }
-      zq[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, sum[nt], 8 * t), __shfl_sync(0xFFFFFFFFu, sum[nt], 8 * t + 4));
+      mul[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, back, 8 * t), __shfl_sync(0xFFFFFFFFu, back, 8 * t + 4));
+      zq[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, sum, 8 * t), __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = k.rt * R + nt * 8 + 2 * t + i;
@@ -299,13 +291,14 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     q.load(a, at, smem + L::kOffQ + q_at * L::kQBytes, lane);
     if (++q_at == kDecQueries) q_at = 0;
     float o[NT][MT][4];
-    float2 m[NT], l[NT], z[NT];
+    float2 m[NT], l[NT], z[NT], unit[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.0f;
       m[nt] = make_float2(kKv4NoMax, kKv4NoMax);
       l[nt] = z[nt] = make_float2(0.0f, 0.0f);
+      unit[nt] = make_float2(1.0f, 1.0f);
     }
     const int kv = min(at.seq.kv, a.c.capacity);
     // tiles from these tokens on are seen whole by every row
@@ -322,7 +315,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
       const __half2* kpar = reinterpret_cast<const __half2*>(buf + kDecTile * HD);
       const __half2* vpar = kpar + kDecTile;
       // S' = K Q': rows g and g + 8 are tokens.  Two chains of sums for each 16 tokens: a chain's products wait for one another
-      float2 x[kPieces][NT][2];  // scores of tokens 16 i + g and 16 i + g + 8, query rows 2t and 2t + 1
+      float2 x[kPieces][NT][2];  // scores of tokens 16 i + g and 16 i + g + 8, query rows 2t and 2t + 1, over q.mul
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         uint32_t ka[W], kb[W];
@@ -351,13 +344,19 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt][v], a0, a1, a2, a3, q.f[nt][2 * w + v][0], q.f[nt][2 * w + v][1]);
           }
         const float2 k0 = __half22float2(kpar[i * 16 + g]), k1 = __half22float2(kpar[i * 16 + g + 8]);
-        const float2 s0 = both(k0.x * q.mul), s1 = both(k1.x * q.mul);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          x[i][nt][0] = __ffma2_rn(s0, __fadd2_rn(make_float2(s[nt][0][0], s[nt][0][1]), make_float2(s[nt][1][0], s[nt][1][1])),
-                                   __fmul2_rn(both(k0.y), q.zq[nt]));
-          x[i][nt][1] = __ffma2_rn(s1, __fadd2_rn(make_float2(s[nt][0][2], s[nt][0][3]), make_float2(s[nt][1][2], s[nt][1][3])),
-                                   __fmul2_rn(both(k1.y), q.zq[nt]));
+          const float2 s0 = __fadd2_rn(make_float2(s[nt][0][0], s[nt][0][1]), make_float2(s[nt][1][0], s[nt][1][1]));
+          const float2 s1 = __fadd2_rn(make_float2(s[nt][0][2], s[nt][0][3]), make_float2(s[nt][1][2], s[nt][1][3]));
+          // (one query tile: scalars, which need no pair made of a scale; two: pairs.  The other way round 222.3 us where this
+          // takes 220.1 on the batch above, and 61.2 where 60.4 for four tokens of 16 x 30000, 16 heads of 64 over 2)
+          if constexpr (NT == 1) {
+            x[i][nt][0] = make_float2(fmaf(k0.x, s0.x, k0.y * q.zq[nt].x), fmaf(k0.x, s0.y, k0.y * q.zq[nt].y));
+            x[i][nt][1] = make_float2(fmaf(k1.x, s1.x, k1.y * q.zq[nt].x), fmaf(k1.x, s1.y, k1.y * q.zq[nt].y));
+          } else {
+            x[i][nt][0] = __ffma2_rn(both(k0.x), s0, __fmul2_rn(both(k0.y), q.zq[nt]));
+            x[i][nt][1] = __ffma2_rn(both(k1.x), s1, __fmul2_rn(both(k1.y), q.zq[nt]));
+          }
         }
       }
       // value scales and zeros, and the exponents of the scales
@@ -398,7 +397,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
         for (int i = 0; i < kPieces; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float2 v = __fadd2_rn(x[i][nt][j], both(ve[i][j]));
+            const float2 v = __ffma2_rn(x[i][nt][j], q.mul[nt], both(ve[i][j]));
             high[nt] = make_float2(fmaxf(high[nt].x, v.x), fmaxf(high[nt].y, v.y));
           }
         lift |= high[nt].x > m[nt].x + 8.0f || high[nt].y > m[nt].y + 8.0f;
@@ -414,6 +413,8 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
           high[nt] = make_float2(fmaxf(high[nt].x, m[nt].x), fmaxf(high[nt].y, m[nt].y));
           const float2 by = make_float2(exp2_approx(m[nt].x - high[nt].x), exp2_approx(m[nt].y - high[nt].y));
           m[nt] = high[nt];
+          kv4_units(m[nt].x, q.mul[nt].x, unit[nt].x);
+          kv4_units(m[nt].y, q.mul[nt].y, unit[nt].y);
           l[nt] = __fmul2_rn(l[nt], by);
           z[nt] = __fmul2_rn(z[nt], by);
 #pragma unroll
@@ -432,7 +433,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
         for (int i = 0; i < kPieces; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float2 y = __fadd2_rn(x[i][nt][j], low);
+            const float2 y = __ffma2_rn(x[i][nt][j], q.mul[nt], low);
             const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
             l[nt] = __fadd2_rn(l[nt], p);
             z[nt] = __ffma2_rn(p, both(vp[i][j].y), z[nt]);
@@ -502,7 +503,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
               make_float4(fmaf(o[nt][2 * j][i], 16777216.0f, zs), fmaf(o[nt][2 * j][2 + i], 1048576.0f, zs),
                           fmaf(o[nt][2 * j + 1][i], 16777216.0f, zs), fmaf(o[nt][2 * j + 1][2 + i], 1048576.0f, zs));
         if (g == 0) {
-          ml[(warp * R + r) * 2] = i ? m[nt].y : m[nt].x;
+          ml[(warp * R + r) * 2] = i ? m[nt].y * unit[nt].y : m[nt].x * unit[nt].x;
           ml[(warp * R + r) * 2 + 1] = ls;
         }
       }
