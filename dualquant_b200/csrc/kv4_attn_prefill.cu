@@ -241,23 +241,21 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
                                          __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
           big = max(big & 0xFFFFu, big >> 16);
           // Ordinary rows, largest element in [2^-10, 2^15), are fp16 as they are (what lies below 2^-14 of them is off by 2^-25
-          // at most); if one of the warp's rows is not, the factors of all of them are looked up.
+          // at most); if one of the warp's rows is not, or the scale is huge, the factors of all of them are looked up.
           const uint32_t small = __ballot_sync(0xFFFFFFFFu, big < 0x3A80u);
           constexpr uint32_t kRowMask = (1u << kRowLanes) - 1u;
-          const bool odd = big >= 0x4700u || ((small >> (lane & ~(kRowLanes - 1))) & kRowMask) == kRowMask;
+          const bool odd = big >= 0x4700u || ((small >> (lane & ~(kRowLanes - 1))) & kRowMask) == kRowMask || fabsf(a.scale2) > 1e12f;
           bool finite_row = true;
-          float by = 1.0f, mul_row = fmaxf(fabsf(a.scale2), 1.2e-38f);
+          float by = a.scale2 > 0.0f ? 1.0f : a.scale2 < 0.0f ? -1.0f : 0.0f;  // (the maximum is taken of scores times |scale|)
+          float mul_row = a.scale2 != 0.0f ? fmaxf(fabsf(a.scale2), 1.2e-38f) : 1.0f;
           if (__any_sync(0xFFFFFFFFu, odd)) {
 #pragma unroll
             for (int d = 1; d < kRowLanes; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
             finite_row = big < 0x7F80u;  // no infinity and no NaN; rows that are not finite are made zero here
-            const int e = big > 0 && finite_row ? static_cast<int>(big >> 7) - 127 : 0;
-            const int up = max(min(14 - e, 100), -103);
-            by = __int_as_float((up + 127) << 23);
-            mul_row = fmaxf(fabsf(a.scale2) * __int_as_float((127 - up) << 23), 1.2e-38f);
+            const Kv4RowScale f = kv4_row_scale(finite_row ? big : 0, a.scale2);
+            by = f.up;
+            mul_row = f.back;
           }
-          if (a.scale2 < 0.0f) by = -by;  // (the maximum is taken of scores times |scale|)
-          if (a.scale2 == 0.0f) by = 0.0f, mul_row = 1.0f;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
