@@ -152,6 +152,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   uint64_t* v_full = k_empty + kPreStages;
   uint64_t* v_empty = v_full + kPreStages;
   uint64_t* s_full = v_empty + kPreStages;      // [row tile] scores of a token tile are in tensor memory
+  // (Of a row tile by itself, scores of the next token tile follow the first half's weights: a warp may bring a second half while
+  // another has yet to bring the one before, and arrivals are counted, not named.  Its second halves therefore take two barriers
+  // in turn, 1 and 3; that of the second half but one is through, since there are scores of this token tile.)
   uint64_t* p_full = s_full + 2;                // [row tile][half] weights of 64 tokens are
   uint64_t* o_done = p_full + 4;                // [row tile][half] the values of its weights are in the output
   float* q_mul = reinterpret_cast<float*>(smem + L::kOffMul);
@@ -212,6 +215,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes, in the upper half of an address
     const uint32_t t_s = tmem + lanes + tile * 128, t_o = tmem + lanes + 256 + tile * HD;
     uint32_t count[2] = {0, 0};  // first and second halves of token tiles so far
+    auto second = [&](uint32_t n) { return kOne ? 1 + 2 * (n & 1) : 2 * tile + 1; };  // barrier of second half n, and its phase
+    auto second_phase = [&](uint32_t n) { return (kOne ? n >> 1 : n) & 1; };
     int seen = 0;          // token tiles of the call, both row tiles'
     uint32_t q_uses = 0;
     bool is_first = true, goes_on = false, fresh = true, more = true;
@@ -285,7 +290,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           // output of the row
           const float l = l2.x + l2.y;
           const int last_half = (pre_groups(a.c, at) - 1) & 1;
-          ok = ok && mbar_wait(o_done + 2 * tile + last_half, ((last_half ? count[1] : count[0]) - 1) & 1, &s_abort, 44);
+          ok = ok && mbar_wait(o_done + (last_half ? second(count[1] - 1) : 2 * tile),
+                               last_half ? second_phase(count[1] - 1) : (count[0] - 1) & 1, &s_abort, 44);
           tc_fence_after();
           const bool whole_segment = at.u0 == 0 && at.u1 == at.span.count;
           // a row that sees no token is zero (and not 0 / 0), one that is not finite NaN
@@ -423,8 +429,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
               // the groups before are in O: of two row tiles those of earlier tiles are since there are scores of this one
-              if (half == 1) ok = ok && mbar_wait(o_done + 2 * tile, (count[0] - 1) & 1, &s_abort, 43);
-              else if (kOne) ok = ok && mbar_wait(o_done + 1, (count[1] - 1) & 1, &s_abort, 46);
+              if (half == 1 || kOne)
+                ok = ok && mbar_wait(o_done + (half == 1 ? 2 * tile : second(count[1] - 1)),
+                                     half == 1 ? (count[0] - 1) & 1 : second_phase(count[1] - 1), &s_abort, 43);
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
@@ -464,12 +471,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           }
           tmem_st_wait();
           tc_fence_before();
-          // Of a row tile by itself, scores of the next token tile follow the first half's weights: a warp may be here again while
-          // another has yet to bring its second half of the tile before, whose arrivals are counted, not named.  So nobody brings a
-          // second half before the last one's products are done (they are, but for a warp that was held up); that also keeps the
-          // phases that are waited for above and behind the segment one apart.
-          if (kOne && half == 1 && j > 1) ok = ok && mbar_wait(o_done + 1, (count[1] - 2) & 1, &s_abort, 57);
-          mbar_arrive(p_full + 2 * tile + half);
+          mbar_arrive(p_full + (half == 0 ? 2 * tile : second(count[1] - 1)));
         }
       }
       more = kv4_next_segment<kPreTile>(a.c, a.m, a.g, ROWS, next);
@@ -628,14 +630,17 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
       };
       auto values = [&](int t, int at_s, uint32_t tile_number, int half, bool add) {
         const uint32_t va = base + L::kOffV + tile_number % kPreStages * L::kOperand + half * 8192;
-        ok = ok && mbar_wait(p_full + 2 * t + half, p_phase[t][half]++ & 1, &s_abort, 51);
+        const uint32_t nth = p_phase[t][half]++;
+        const bool turns = kOne && half == 1;
+        const int bar_at = turns ? 1 + 2 * (nth & 1) : 2 * t + half;
+        ok = ok && mbar_wait(p_full + bar_at, (turns ? nth >> 1 : nth) & 1, &s_abort, 51);
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           pre_mma_ts(tmem + 256 + t * HD, tmem + at_s * 128 + half * 64 + k * 8, pre_desc_rows(va + k * 2048, L::kHalf), kIdescO,
                      add || k > 0);
-        umma_commit(o_done + 2 * t + half);
+        umma_commit(o_done + bar_at);
       };
       // Of two row tiles, a tile's next scores follow its weights' second half: products run in order, so those weights have been
       // read.  A row tile by itself has the other's scores' columns for every second token tile; its next scores follow its
