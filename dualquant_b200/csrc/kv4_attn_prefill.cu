@@ -221,7 +221,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
     uint32_t q_uses = 0;
     bool is_first = true, goes_on = false, fresh = true, more = true;
     Kv4Cursor next = at;
-    float mul = 1.0f, m = kKv4NoMax;
+    float mul = 1.0f, m = kKv4NoMax, unit = 1.0f;
     float2 l2 = make_float2(0.0f, 0.0f);
     bool finite = true;
     // One round: the queries of the next segment, so that its scores are computed meanwhile; the output of this segment; the
@@ -348,7 +348,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
             }
           }
           if (!whole_segment && there) {
-            part[2 * (tile * 128 + row_in)] = m;
+            part[2 * (tile * 128 + row_in)] = m * unit;
             part[2 * (tile * 128 + row_in) + 1] = l;
           }
           tc_fence_before();  // (the next segment's products over O come behind this row's next arrival)
@@ -385,6 +385,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
         l2 = make_float2(0.0f, 0.0f);
         finite = !isnan(mul_next);
         mul = finite ? mul_next : 1.0f;
+        unit = 1.0f;
         // groups from these tokens on are seen whole by every row
         const int whole_hi = min(kv, at.span.p_lo + 1) - 64, whole_lo = a.m.window > 0 ? at.span.p_hi - a.m.window : -1,
                   whole_sinks = a.m.window > 0 ? a.m.sinks - 64 : -1;
@@ -426,6 +427,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
           if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
             const float to = fmaxf(m, high), by = pre_exp2(m - to);
             m = to;
+            kv4_units(m, mul, unit);
             l2 = make_float2(l2.x * by, l2.y * by);
             if (j > 0) {
               // the groups before are in O: of two row tiles those of earlier tiles are since there are scores of this one
