@@ -136,7 +136,6 @@ __device__ __forceinline__ int pre_groups(const Kv4Batch& c, const Kv4Cursor& k)
 template <int HD, int ROWS>
 __global__ void __launch_bounds__(kPreThreads, 1)
 kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
-  grid_dep_launch_dependents();
   using L = PreSmem<HD>;
   constexpr bool kOne = ROWS == 128;  // segments of one row tile
   extern __shared__ uint8_t smem_raw[];
@@ -186,6 +185,8 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* status) {
   if (warp == 12) {
     tmem_alloc(s_tmem, 512);
     tmem_relinquish();
+    // Behind the allocation: a kernel that came first on this SM could hold tensor memory until this one is done.
+    grid_dep_launch_dependents();
   }
   grid_dep_wait();
   if (warp == 0) {
