@@ -494,15 +494,18 @@ class Decoder:
         return run
 
     def decode_step(self, ids: torch.Tensor, pos_t: torch.Tensor) -> torch.Tensor:
-        """ids [B] (one token per sequence), pos_t: int64 device tensor [1] with the cache position.
-        Everything is indexed through pos_t, so the step can be captured in a CUDA graph."""
+        """ids [B] (one token per sequence), pos_t: int64 device tensor [1] with the cache position (with the paged
+        cache also [B], one for each sequence).  Everything is indexed through pos_t, so the step can be captured in a
+        CUDA graph.  With the paged cache a step at a position outside of it stores nothing, and its logits are NaN."""
         x = self.embed[ids].unsqueeze(1)
         if self.paged is not None:
-            kv_len = (pos_t + 1).to(torch.int32).expand(ids.shape[0]).contiguous()
+            # positions outside of the cache become -1 or max_len, and their length, 0 or max_len + 1, becomes 0
+            at = pos_t.clamp(-1, self.max_len).to(torch.int32)
+            kv_len = (at.expand(ids.shape[0]) + 1).remainder_(self.max_len + 1)
             for layer in self.layers:
                 x = layer.forward(x, None, None, 0, pos_t, None, self.group, self.ar, kv_len=kv_len)
             x = _rms_norm(x[:, 0], self.norm, self.cfg.rms_norm_eps)
-            return x @ self.lm_head.T
+            return (x @ self.lm_head.T).masked_fill_((kv_len == 0)[:, None], float("nan"))
         cos = self.cos.index_select(0, pos_t)
         sin = self.sin.index_select(0, pos_t)
         # additive mask over the unwritten tail of the cache, built once per step (a boolean mask
