@@ -398,9 +398,12 @@ class Decoder:
         B, S = ids.shape
         if pos0 and self.paged is None:
             raise ValueError("prompts in pieces need the paged cache (kv='int4')")
+        self._check_positions(pos0, S)
+        return self._prefill_tail(self._prefill_body(ids, pos0), B, S)
+
+    def _check_positions(self, pos0: int, S: int):
         if pos0 < 0 or pos0 + S > self.max_len:
             raise ValueError(f"positions {pos0} .. {pos0 + S - 1} outside of the cache of {self.max_len}")
-        return self._prefill_tail(self._prefill_body(ids, pos0), B, S)
 
     def _token_sharded(self, B: int, S: int) -> bool:
         return self.tp > 1 and self.token_sharded_prefill and (B * S) % self.tp == 0
@@ -468,6 +471,7 @@ class Decoder:
         parallelism over NCCL) nothing is captured and run() is the eager prefill.  With the
         peer-memory exchange all ranks must capture and replay together."""
         B, S = ids.shape
+        self._check_positions(0, S)
         if self.tp > 1 and not self._peer_exchange(B, S):
             return lambda new_ids=None: self.prefill(ids if new_ids is None else new_ids)
         static_ids = ids.clone()

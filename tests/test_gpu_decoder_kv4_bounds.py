@@ -1,4 +1,4 @@
-"""Decoder with the paged 4-bit cache: steps that pass the cache's end."""
+"""Decoder with the paged 4-bit cache: steps and prompts that pass the cache's end."""
 import pytest
 import torch
 
@@ -66,3 +66,14 @@ def test_a_position_outside_of_the_cache_of_one_sequence_keeps_to_it():
         m.prefill(ids)
         out = m.decode_step(ids[:, 0], torch.tensor([10, 12], device=DEV))
         assert bool(out[0].isfinite().all()) and bool(out[1].isnan().all())
+
+
+@pytest.mark.parametrize("kv", ["int4", "bf16"])
+def test_a_captured_prompt_longer_than_the_cache_is_refused(kv):
+    m = make(1)
+    ids = torch.zeros(1, 33, dtype=torch.long, device=DEV)
+    with torch.no_grad():
+        m.alloc_cache(1, 32, kv=kv)
+        with pytest.raises(ValueError):
+            m.capture_prefill(ids)
+        m.capture_prefill(ids[:, :32])()
