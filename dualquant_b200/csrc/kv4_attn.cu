@@ -178,7 +178,8 @@ extern "C" int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, i
   DQ_REQUIRE(static_cast<int64_t>(a.c.T) * hq < (1ll << 30), DQ_ERR_SHAPE, "%d rows of %d heads", a.c.T, hq);
   DQ_REQUIRE(q_row_stride % 8 == 0 && q_head_stride % 8 == 0 && aligned(q_bf16, 16) && aligned(out_bf16, 16), DQ_ERR_ALIGN,
              "query heads and outputs must be 16-byte aligned");
-  DQ_REQUIRE(isfinite(scale), DQ_ERR_SHAPE, "scale is not finite");
+  const float scale2 = scale * 1.4426950408889634f;
+  DQ_REQUIRE(isfinite(scale2), DQ_ERR_SHAPE, "scale log2(e) is not finite");
   a.g.G = hq / a.c.hkv;
   const int hd = batch->head_dim;
   const Kv4Plan p = kv4_plan(a.c, a.g.G, hd, max_new, st);
@@ -196,7 +197,7 @@ extern "C" int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, i
   a.grid = kv4_div(p.grid);
   a.join = static_cast<Kv4Join*>(workspace);
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.join_bytes);
-  a.scale2 = scale * 1.4426950408889634f;
+  a.scale2 = scale2;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   rc = p.R >= 128 ? launch_kv4_prefill(a, hd, p.R, p.grid, cs, st) : launch_kv4_decode(a, hd, p.R, p.grid, cs);
   if (rc != DQ_OK || p.grid == 1) return rc;

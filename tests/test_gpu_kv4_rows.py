@@ -18,8 +18,8 @@ def i32(v):
 
 # (new tokens, most rows that a sequence is said to bring): four heads a group, so tiles of 8 and 16 rows
 TILES = [pytest.param([1, 2], 2, id="8"), pytest.param([4, 3], 4, id="16")]
-# ... and of 128 and 256, whose keys are rounded to fp16
-MANY = [pytest.param([5, 2], 20, id="128"), pytest.param([9, 2], 100, id="256")]
+# ... and of 128 and 256, whose keys are rounded to fp16 (no more rows count than the call has tokens)
+MANY = [pytest.param([9, 3], 12, id="128"), pytest.param([30, 13], 43, id="256")]
 
 
 def taken(ks, most):
@@ -35,11 +35,13 @@ def test_a_row_of_large_finite_queries_leaves_its_neighbours_as_they_are(hd, new
     lengths = [400, 77]
     pages, table, ks, vs = ref.make_cache(gen, 2, lengths, 1, hd, 16)
     q = torch.randn(sum(new), 4, hd, generator=gen).to(torch.bfloat16).cuda()
-    # head 1 of the first token sees one key far above all others: its own row is that token's values
-    one = 37
-    q[0, 1] = (ks[0][0, one].sign() * size).to(torch.bfloat16)
-    score = ks[0][0, : lengths[0] - new[0] + 1] @ q[0, 1].double()
-    assert int(score.argmax()) == one and float(score.topk(2).values.diff()) < -0.1 * float(score.abs().max())
+    # head 1 of the first token has the signs of the key with the largest sum of sizes, which no other key's score reaches: its own
+    # row is that token's values (a gap of 2^-10 of the score is 2^10 times what fp32 resolves, and above 1000 at 1e7)
+    seen = ks[0][0, : lengths[0] - new[0] + 1]
+    one = int(seen.abs().sum(-1).argmax())
+    q[0, 1] = (seen[one].sign() * size).to(torch.bfloat16)
+    score = seen @ q[0, 1].double()
+    assert int(score.argmax()) == one and float(score.topk(2).values.diff()) < -(2.0 ** -10) * float(score.abs().max())
     got = ops.kv4_attention(q, ops.KV4Cache(pages, hd, 16), table, i32(lengths), cu_of(new), most)
     want = ref.attention(q, taken(ks, most), vs, new, lengths)
     tol = ref.attention_tolerance(want, vs, lengths)
@@ -89,3 +91,37 @@ def test_scores_that_grow_to_any_size(hd, new, most, size):
     # neighbouring levels may both count where scores are small (0.1 * 128 / sqrt(128) and 8 times that)
     assert bool(((got.double() - want).abs() <= ref.attention_tolerance(want, vs, lengths)).all())
     _lib.device_status(0)
+
+
+@pytest.mark.parametrize("most", [1, 12, 43])
+def test_scales_up_to_the_largest_and_refusal_of_larger_ones(most):
+    gen = torch.Generator().manual_seed(3)
+    pages, table, ks, vs = ref.make_cache(gen, 1, [90], 1, 64, 16)
+    q = (torch.randn(most, 4, 64, generator=gen).double() * 1e-38).to(torch.bfloat16).cuda()
+    cache, n = ops.KV4Cache(pages, 64, 16), i32([90])
+    for scale in (3.4e38, -3.4e38, 2.4e38):  # times log2(e): past the largest number of fp32
+        with pytest.raises(ValueError):
+            ops.kv4_attention(q, cache, table, n, max_new=most, scale=scale)
+    for scale in (2.3e38, -2.3e38):
+        got = ops.kv4_attention(q, cache, table, n, max_new=most, scale=scale)
+        want = ref.attention(q, taken(ks, most), vs, [most], [90], scale=scale)
+        # scores of up to 60 or so: within the 64 that the tolerance counts on
+        assert bool(((got.double() - want).abs() <= ref.attention_tolerance(want, vs, [90])).all())
+
+
+@pytest.mark.parametrize("q_scale", [1.5, 5.0, 20.0])
+@pytest.mark.parametrize("new,most", MANY)
+def test_rounded_keys_move_a_row_by_no_more_than_their_rounding(new, most, q_scale):
+    """Against the definition, with keys as the cache holds them: fp16 is off by 2^-11 of an element, a score by up to d of
+    them, and weights of scores that are off by d each lie within exp(+-2 d) of theirs."""
+    gen = torch.Generator().manual_seed(most)
+    hd, lengths = 128, [700, 90]
+    pages, table, ks, vs = ref.make_cache(gen, 2, lengths, 1, hd, 32)
+    q = (torch.randn(sum(new), 4, hd, generator=gen) * q_scale).to(torch.bfloat16).cuda()
+    got = ops.kv4_attention(q, ops.KV4Cache(pages, hd, 32), table, i32(lengths), cu_of(new), most)
+    want = ref.attention(q, ks, vs, new, lengths)
+    d = torch.cat([torch.einsum("ihd,jd->ihj", q[a : a + n].double().abs(), k[0].abs()).amax(-1)
+                   for a, n, k in zip((0, new[0]), new, ks)]) * hd ** -0.5 * 2.0 ** -11
+    span = max(float((v.amax(-1) - v.amin(-1)).max()) for v in vs)
+    tol = ref.attention_tolerance(want, vs, lengths) + span * (torch.expm1(2 * d)[..., None] + 8.3 * q_scale * 2.0 ** -20)
+    assert bool(((got.double() - want).abs() <= tol).all())
