@@ -118,10 +118,15 @@ struct Kv4Plan {
 static Kv4Plan kv4_plan(const Kv4Batch& c, int G, int hd, int max_new, DeviceState* st) {
   Kv4Plan p;
   const int64_t rows = static_cast<int64_t>(G) * max_new;
-  // The few-rows kernel reads the cache once for every 16 rows, the other one once for up to 128 or 256.  32 heads of 128 over 8,
-  // us: 16, 32, 48, 64 rows over 16 x 4000 tokens 36, 58, 82, 100 in tiles of 16, and 61 to 62 for 48 and 64 in one of 128; over
-  // 8 x 30000 tokens 83, 150, 219, 286 and 184 to 185; over 1 x 4000 14, 20, 22, 23 and 16 to 17.  A row tile of 128 by itself
-  // in the two-tile kernel: 72, 218 and 17.
+  // The few-rows kernel reads the cache once for every 8 or 16 rows, the other one once for up to 128 or 256.  32 heads over 8, us:
+  //                 tokens         8 rows by 8, 16   16 by 8, 16    32 by 16, 128   48 by 16, 128   64 by 16, 128
+  //   heads of 128  16 x 4000         27   33          42   37         58   61         82   62         99   63
+  //                  8 x 30000        61   79         110   83        148  184        215  186        279  187
+  //                  1 x 4000         11              13   14         20              22   17         24   17
+  //   heads of 64   16 x 4000         20   24          32   27         44   53         60   54         72   55
+  //                  8 x 30000        44   57          77   60        107  163        155  163        201  164
+  //                  1 x 4000          9              11   11         16              17   14         19   14
+  // A row tile of 128 by itself in the two-tile kernel: 72, 218 and 17 (heads of 128).
   p.R = rows <= 8 ? 8 : rows <= 32 ? 16 : rows <= 128 ? 128 : 256;
   const bool many = p.R >= 128;
   const int tile = many ? kPreTile : kDecTile, least = many ? kPreLeast : kDecLeast;

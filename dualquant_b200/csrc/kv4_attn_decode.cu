@@ -18,14 +18,16 @@
 // sequences of up to 8000 tokens, 265 and 257 on the batch below, at that stage.)
 // Weights and sums:
 //   * p_j s_j is fp16 (an mma operand, 2^-11 relative, in the row's own scale): the reference point m is taken of
-//     x_j + exponent(s_j), so that p_j s_j stays below 2^9 and what counts stays normal whatever the scales are;
+//     x_j + exponent(s_j), so that p_j s_j stays below 2^10 and what counts stays normal whatever the scales are.  The rounding
+//     meets codes 0 ... 15 and not the centred values: outputs are up to 17 % further from 64 bits than their bf16 rounding is;
 //   * m moves only where a row would pass 2^8 above it; l, sum p z and O are fp32.
 // Query rows are fp16 times a power of two of the row: an element is exact down to 2^-27 of the row's largest one (fp16 has its
 // 8 bits down to 2^-17, every other element is taken times 1 / 16), and no row knows of its neighbours.
 //
-// 64 sequences of up to 16384 tokens, 8 heads of 128, four rows each: 1.14 GB in 219 us, 5.2 TB/s, 81 % of what a plain copy
-// moves.  The integer pipe is nearest to its end there (59 % of its cycles, issue slots 55 %): ANDs and shifts that take the
-// codes apart, which twelve warps an SM cannot overlap any better.  Small batches pay for the launch, a first look at cold instructions, three
+// 64 sequences of up to 16384 tokens, 8 heads of 128, four rows each, 1.14 GB: 220 us replayed from a graph (5.2 TB/s, 80 % of
+// what a plain copy moves), 249 us a call when the inputs change from call to call (71 %).  No unit is at its end (integer pipe 60 %
+// of its cycles, issue slots 56 %, memory 61 %): the twelve warps of an SM wait for their own results of fixed latency, 1.4
+// cycles an issue.  Small batches pay for the launch, a first look at cold instructions, three
 // dependent loads (lengths, pages, codes) and the second kernel: 9.3 us for one row over 300 tokens.  Four CTAs an SM at 128
 // registers, three stages at two CTAs an SM, and tiles of 64 tokens were no faster.
 #include "kv4.cuh"

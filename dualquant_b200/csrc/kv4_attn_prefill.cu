@@ -17,9 +17,10 @@
 // Keys, values and queries hold the elements of each group of eight in the order 0 4 1 5 2 6 3 7, in which nibbles come out of a
 // word two at a time; outputs undo it.  The running maximum m moves only where a row would pass 2^8 above it.
 //
-// Eight prompts of 2048 tokens, 32 heads of 128 over 8: 275 GFLOP in 410 us, 670 TFLOP/s, 40 % of the rate of a plain matrix
-// product.  Neither memory (7 %) nor the tensor cores (38 % of their cycles) bound that, but the issue slots of sixteen warps (half
-// of them busy) and the way of a tile through them: score, maximum, weight, product.  Without any arithmetic on the scores the
+// Eight prompts of 2048 tokens, 32 heads of 128 over 8, 275 GFLOP: 409 us replayed from a graph (670 TFLOP/s, 41 % of the rate of
+// a plain matrix product), 432 us a call when the inputs change from call to call (640, 39 %).  Neither memory (8 %) nor the
+// tensor cores (36 % of their cycles) nor issue slots (51 %) are at their end: what bounds it is the dependent way of a tile,
+// score, maximum, weight, product, of which a row tile has one at a time.  Without any arithmetic on the scores the
 // same waits and products take 305 us.  The first tile of a segment waits for its queries and the last for its output, 10000
 // cycles a segment: the softmax warps therefore convert the next queries before they write outputs.  Scores of a whole tile in
 // a thread's registers spilled and left the instruction cache; they are taken by halves, and loops are kept short.

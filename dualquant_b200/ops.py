@@ -677,7 +677,7 @@ def kv4_append(qkv: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tensor, 
     first row of each sequence's new tokens (None: T / B rows each).  Row i of a sequence with n new tokens goes to position
     kv_len - n + i.  cos_tab / sin_tab fp32 [positions, d / 2].  rotate: a normalised Walsh-Hadamard rotation over the head of
     queries and keys behind the position rotation, which spreads outlier channels of keys over the 4-bit grid and leaves
-    q . k as it is.  All index tensors are read on the device; rows from cu_new[B] on are left as they were.  A token without
+    q . k as it is.  All index tensors are read on the device; rows from cu_new[B] on are not written.  A token without
     a place (negative position, behind the table row or the rotation tables) gets a zero query row and is not written, nor is
     one whose page number lies outside of the cache.  No two tokens of a call may have the same slot of a page: either could
     stay."""
@@ -687,7 +687,8 @@ def kv4_append(qkv: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tensor, 
 def kv4_read(cache: KV4Cache, block_table: torch.Tensor, kv_len: torch.Tensor, tokens: int,
              cu_new: Optional[torch.Tensor] = None):
     """What the cache holds for the last tokens of each sequence (rows as in kv4_append, `tokens` of them in all):
-    (keys, values) bf16 [tokens, hkv, d], keys as they were stored (rotated).  Tokens that are not there are zero."""
+    (keys, values) bf16 [tokens, hkv, d], keys as they were stored (rotated).  Tokens that are not there are zero; rows from
+    cu_new[B] on are not written."""
     return _lib.host().kv4_read(cache, block_table, kv_len, tokens, cu_new)
 
 
@@ -696,8 +697,11 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, k
                   scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal grouped-query attention of the new tokens (q [T, hq, d] bf16, rows as in kv4_append) over the paged 4-bit cache:
     bf16 [T, hq, d].  window > 0: a token sees itself, the window - 1 tokens before it and the first `sinks` tokens of its
-    sequence.  scale: default d ** -0.5.  max_new: the most rows that a sequence brings, which chooses the kernel; T (or T / B
-    without cu_new) if not given.  A row that sees no token is zero; rows from cu_new[B] on are not written.  With more than 32
-    rows to a key/value head (hq / hkv * max_new) keys and values are rounded to fp16 (2^-11 of the number), with fewer the
-    products are taken of the codes themselves."""
+    sequence.  scale: default d ** -0.5; its product with log2(e) must be finite in fp32.  max_new: the most rows that a sequence
+    brings, which chooses the kernel; T (or T / B without cu_new) if not given.  Give it with cu_new: a batch of single tokens
+    without it runs on the kernel for prompts, two to four times slower.  A row that sees no token is zero, one that is not
+    finite NaN; rows from cu_new[B] on are not written.  With more than 32 rows to a key/value head (hq / hkv * max_new) keys and values
+    are rounded to fp16 (2^-11 of the number; a score then moves by up to that of sum |q| |k| scale, a weight by as much of
+    itself), with fewer the products are taken of the codes themselves.  Pages must stand for numbers that fp16 holds, as
+    kv4_append leaves them."""
     return _lib.host().kv4_attention(q, cache, block_table, kv_len, cu_new, max_new, window, sinks, scale, out)

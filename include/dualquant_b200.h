@@ -622,10 +622,11 @@ DQ_API int dq_kv4_append(const dq_kv4_batch* batch, const void* qkv_bf16, int64_
 DQ_API int dq_kv4_read(const dq_kv4_batch* batch, void* k_out_bf16, void* v_out_bf16, void* stream);
 /* Causal attention of the new tokens over the cache: hq query heads in groups of hq / hkv, q [tokens][hq][head_dim] bf16 with
  * the given strides (elements).  window > 0: a token sees itself, the window - 1 tokens before it and the first `sinks`
- * tokens of its sequence.  max_new: no sequence brings more rows (a hint; more are computed all the same).  A row that sees
- * nothing is zero.  out [tokens][hq][head_dim] bf16.  Groups of up to 32 rows (hq / hkv * max_new) multiply with the codes
- * themselves; with more rows keys and values are scale * c + zero rounded to fp16 (2^-11 of the number).  cu_new must not
- * decrease: of a batch in which it does, rows may be left out. */
+ * tokens of its sequence.  max_new: no sequence brings more rows (a hint that chooses the kernel; more are computed all the
+ * same).  A row that sees nothing is zero, one that is not finite NaN; queries of any finite size keep to their own row.
+ * scale log2(e) must be finite.  out [tokens][hq][head_dim] bf16.  Groups of up to 32 rows (hq / hkv * max_new) multiply with the codes
+ * themselves; with more rows keys and values are scale * c + zero rounded to fp16 (2^-11 of the number), which must be finite
+ * there, as dq_kv4_append leaves them.  cu_new must not decrease: of a batch in which it does, rows may be left out. */
 DQ_API size_t dq_kv4_attention_workspace_bytes(const dq_kv4_batch* batch, int hq, int max_new);
 DQ_API int dq_kv4_attention(const dq_kv4_batch* batch, const void* q_bf16, int64_t q_row_stride, int64_t q_head_stride,
                             int hq, int max_new, int window, int sinks, float scale, void* out_bf16, void* workspace,
